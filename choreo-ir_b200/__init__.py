@@ -77,6 +77,47 @@ class DeviceProps(C.Structure):
     ]
 
 
+class FfnDesc(C.Structure):
+    _fields_ = [
+        ("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64), ("dtype", C.c_int32), ("act", C.c_int32),
+        ("x", C.c_void_p), ("ldx", C.c_int64), ("w_gate", C.c_void_p), ("w_up", C.c_void_p), ("ldw", C.c_int64),
+        ("trans_w", C.c_int32), ("reserved", C.c_int32), ("h", C.c_void_p), ("ldh", C.c_int64),
+        ("gate", C.c_void_p), ("up", C.c_void_p), ("ld_gu", C.c_int64),
+    ]
+
+
+class FfnGradDesc(C.Structure):
+    _fields_ = [
+        ("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64), ("dtype", C.c_int32), ("act", C.c_int32),
+        ("x", C.c_void_p), ("ldx", C.c_int64), ("w_gate", C.c_void_p), ("w_up", C.c_void_p), ("ldw", C.c_int64),
+        ("trans_w", C.c_int32), ("dtype_dw", C.c_int32), ("dh", C.c_void_p), ("ld_dh", C.c_int64),
+        ("gate", C.c_void_p), ("up", C.c_void_p), ("ld_gu", C.c_int64), ("dx", C.c_void_p), ("ld_dx", C.c_int64),
+        ("dw_gate", C.c_void_p), ("dw_up", C.c_void_p), ("ld_dw", C.c_int64), ("accumulate_dw", C.c_int32),
+        ("reserved", C.c_int32), ("h", C.c_void_p), ("ldh", C.c_int64),
+    ]
+
+
+class QuantDesc(C.Structure):
+    _fields_ = [
+        ("rows", C.c_int64), ("cols", C.c_int64), ("dtype", C.c_int32), ("transpose", C.c_int32),
+        ("x", C.c_void_p), ("ldx", C.c_int64), ("block_rows", C.c_int32), ("reserved", C.c_int32),
+        ("q", C.c_void_p), ("ldq", C.c_int64), ("scale", C.c_void_p), ("scale_row", C.c_int64),
+        ("scale_blk", C.c_int64),
+    ]
+
+
+class GemmBlockDesc(C.Structure):
+    _fields_ = [
+        ("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64), ("a", C.c_void_p), ("lda", C.c_int64),
+        ("scale_a", C.c_void_p), ("scale_a_row", C.c_int64), ("scale_a_blk", C.c_int64),
+        ("b", C.c_void_p), ("ldb", C.c_int64),
+        ("scale_b", C.c_void_p), ("scale_b_row", C.c_int64), ("scale_b_blk", C.c_int64),
+        ("block_b", C.c_int32), ("dtype_c", C.c_int32), ("c", C.c_void_p), ("ldc", C.c_int64),
+        ("alpha", C.c_float), ("beta", C.c_float), ("addend", C.c_void_p), ("ld_addend", C.c_int64),
+        ("bias", C.c_void_p), ("dtype_bias", C.c_int32), ("relu", C.c_int32),
+    ]
+
+
 # Every symbol include/choreo_b200.h declares, with its ctypes signature.
 _SIGNATURES = {
     "choreo_version": (C.c_int, []),
@@ -103,6 +144,13 @@ _SIGNATURES = {
     "choreo_host_plan_info_get": (C.c_int, [C.c_void_p, C.c_void_p]),
     "choreo_host_plan_part": (C.c_int, [C.c_void_p, C.c_int32, C.POINTER(C.c_int64), C.POINTER(C.c_int64)]),
     "choreo_host_plan_destroy": (C.c_int, [C.c_void_p]),
+    "choreo_gated_ffn_query": (C.c_int, [C.POINTER(FfnDesc), C.POINTER(LaunchConfig)]),
+    "choreo_gated_ffn": (C.c_int, [C.POINTER(FfnDesc), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "choreo_gated_ffn_backward_query": (C.c_int, [C.POINTER(FfnGradDesc), C.POINTER(LaunchConfig)]),
+    "choreo_gated_ffn_backward": (C.c_int, [C.POINTER(FfnGradDesc), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "choreo_quantize_block": (C.c_int, [C.POINTER(QuantDesc), C.c_void_p]),
+    "choreo_gemm_block_scaled_query": (C.c_int, [C.POINTER(GemmBlockDesc), C.POINTER(LaunchConfig)]),
+    "choreo_gemm_block_scaled": (C.c_int, [C.POINTER(GemmBlockDesc), C.c_void_p]),
     "choreo_conv2d": (C.c_int, [C.POINTER(ConvDesc), C.c_void_p, C.c_size_t, C.c_void_p]),
     "choreo_relu": (C.c_int, [C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
     "choreo_add": (C.c_int, [C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
@@ -397,6 +445,201 @@ def fill(x, value: float, stream=None) -> None:
 def convert(src, dst, stream=None) -> None:
     check(lib.choreo_convert(dtype_code(src), src.data_ptr(), dtype_code(dst), dst.data_ptr(), src.numel(),
                              _stream_ptr(stream)))
+
+
+ACT_SILU, ACT_GELU, ACT_GELU_TANH, ACT_RELU = 0, 1, 2, 3
+_ACTS = {"silu": ACT_SILU, "gelu": ACT_GELU, "gelu_tanh": ACT_GELU_TANH, "relu": ACT_RELU}
+
+
+def _matrix(t, rows, cols, name, like=None):
+    """A rows x cols torch matrix with contiguous rows; its leading dimension."""
+    if t.dim() != 2 or tuple(t.shape) != (rows, cols):
+        raise ValueError(f"{name}: expected a {rows} x {cols} matrix, got {tuple(t.shape)}")
+    if t.stride(1) != 1 and cols > 1:
+        raise ValueError(f"{name}: innermost dimension must be contiguous")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise ValueError(f"{name}: dtype and device must be {like.dtype} on {like.device}")
+    return max(t.stride(0), cols) if rows == 1 else t.stride(0)
+
+
+def _act_code(act):
+    if act not in _ACTS:
+        raise ValueError(f"unknown activation {act!r}: one of {', '.join(_ACTS)}")
+    return _ACTS[act]
+
+
+def _workspace(need, workspace, device):
+    """(tensor, bytes): the caller's workspace, or one of `need` bytes."""
+    if workspace is None:
+        if not need:
+            return None, 0
+        import torch
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    return workspace, workspace.numel() * workspace.element_size()
+
+
+def ffn_desc(x, w_gate, w_up, h, *, act="silu", trans_w=False, gate=None, up=None) -> FfnDesc:
+    d = FfnDesc()
+    d.m, d.k = x.shape
+    d.n = w_gate.shape[0] if trans_w else w_gate.shape[1]
+    wshape = (d.n, d.k) if trans_w else (d.k, d.n)
+    d.dtype, d.act, d.trans_w = dtype_code(x), _act_code(act), int(trans_w)
+    d.ldx = _matrix(x, d.m, d.k, "x")
+    d.ldw = _matrix(w_gate, *wshape, "w_gate", x)
+    if _matrix(w_up, *wshape, "w_up", x) != d.ldw:
+        raise ValueError("w_gate and w_up must have the same row stride")
+    d.ldh = _matrix(h, d.m, d.n, "h", x)
+    d.x, d.w_gate, d.w_up, d.h = _ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(h)
+    d.gate, d.up = _ptr(gate), _ptr(up)
+    if gate is not None:
+        d.ld_gu = _matrix(gate, d.m, d.n, "gate", x)
+    if up is not None and _matrix(up, d.m, d.n, "up", x) != d.ld_gu and gate is not None:
+        raise ValueError("gate and up must have the same row stride")
+    return d
+
+
+def gated_ffn_query(d: FfnDesc) -> LaunchConfig:
+    out = LaunchConfig()
+    check(lib.choreo_gated_ffn_query(C.byref(d), C.byref(out)))
+    return out
+
+
+def gated_ffn(x, w_gate, w_up, h, *, act="silu", trans_w=False, gate=None, up=None, workspace=None,
+              stream=None) -> None:
+    """h = act(x @ w_gate) * (x @ w_up) in one kernel; act is "silu", "gelu",
+    "gelu_tanh" or "relu".
+
+    x is M x K and h M x N; the weights are K x N, or N x K with trans_w. gate
+    and up, when given, receive the two products for gated_ffn_backward. Rows
+    may be padded. All are f16, or all bf16."""
+    d = ffn_desc(x, w_gate, w_up, h, act=act, trans_w=trans_w, gate=gate, up=up)
+    need = gated_ffn_query(d).workspace_bytes if workspace is None else 0
+    workspace, ws_bytes = _workspace(need, workspace, h.device)
+    check(lib.choreo_gated_ffn(C.byref(d), _ptr(workspace), ws_bytes, _stream_ptr(stream)))
+
+
+def ffn_grad_desc(dh, x, w_gate, w_up, *, dx=None, dw_gate=None, dw_up=None, gate=None, up=None, h=None, act="silu",
+                  trans_w=False, accumulate=False) -> FfnGradDesc:
+    d = FfnGradDesc()
+    d.m, d.k = x.shape
+    d.n = dh.shape[1]
+    wshape = (d.n, d.k) if trans_w else (d.k, d.n)
+    d.dtype, d.act, d.trans_w = dtype_code(x), _act_code(act), int(trans_w)
+    d.ldx = _matrix(x, d.m, d.k, "x")
+    d.ldw = _matrix(w_gate, *wshape, "w_gate", x)
+    if _matrix(w_up, *wshape, "w_up", x) != d.ldw:
+        raise ValueError("w_gate and w_up must have the same row stride")
+    d.ld_dh = _matrix(dh, d.m, d.n, "dh", x)
+    d.x, d.w_gate, d.w_up, d.dh = _ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(dh)
+    d.gate, d.up, d.dx, d.dw_gate, d.dw_up, d.h = map(_ptr, (gate, up, dx, dw_gate, dw_up, h))
+    if gate is not None:
+        d.ld_gu = _matrix(gate, d.m, d.n, "gate", x)
+    if up is not None and _matrix(up, d.m, d.n, "up", x) != d.ld_gu and gate is not None:
+        raise ValueError("gate and up must have the same row stride")
+    if dx is not None:
+        d.ld_dx = _matrix(dx, d.m, d.k, "dx", x)
+    d.dtype_dw = d.dtype
+    if dw_gate is not None:
+        d.ld_dw = _matrix(dw_gate, *wshape, "dw_gate")
+        d.dtype_dw = dtype_code(dw_gate)
+    if dw_up is not None and _matrix(dw_up, *wshape, "dw_up", dw_gate) != d.ld_dw and dw_gate is not None:
+        raise ValueError("dw_gate and dw_up must have the same row stride")
+    if h is not None:
+        d.ldh = _matrix(h, d.m, d.n, "h", x)
+    d.accumulate_dw = int(accumulate)
+    return d
+
+
+def gated_ffn_backward_query(d: FfnGradDesc) -> LaunchConfig:
+    out = LaunchConfig()
+    check(lib.choreo_gated_ffn_backward_query(C.byref(d), C.byref(out)))
+    return out
+
+
+def gated_ffn_backward(dh, x, w_gate, w_up, *, dx=None, dw_gate=None, dw_up=None, gate=None, up=None, h=None,
+                       act="silu", trans_w=False, accumulate=False, workspace=None, stream=None) -> None:
+    """Gradients of gated_ffn from dh, the gradient of h: dx, dw_gate and dw_up
+    (each pair or dx may be left out). gate and up are what the forward call
+    kept; without them they are computed again from x. h receives h again.
+    The weight gradients may be f32; accumulate adds to what they hold."""
+    d = ffn_grad_desc(dh, x, w_gate, w_up, dx=dx, dw_gate=dw_gate, dw_up=dw_up, gate=gate, up=up, h=h, act=act,
+                      trans_w=trans_w, accumulate=accumulate)
+    need = gated_ffn_backward_query(d).workspace_bytes if workspace is None else 0
+    workspace, ws_bytes = _workspace(need, workspace, dh.device)
+    check(lib.choreo_gated_ffn_backward(C.byref(d), _ptr(workspace), ws_bytes, _stream_ptr(stream)))
+
+
+def _e4m3_matrix(t, rows, cols, name):
+    import torch
+    if t.dtype not in (torch.float8_e4m3fn, torch.uint8):
+        raise ValueError(f"{name}: e4m3 elements (torch.float8_e4m3fn or uint8) required, got {t.dtype}")
+    return _matrix(t, rows, cols, name)
+
+
+def _scales(t, rows, blocks, name):
+    import torch
+    if t.dtype != torch.float32 or tuple(t.shape) != (rows, blocks):
+        raise ValueError(f"{name}: expected f32 scales {rows} x {blocks}, got {t.dtype} {tuple(t.shape)}")
+    return t.stride(0), t.stride(1)
+
+
+def quantize_block(x, q, scale, *, block_rows=1, transpose=False, stream=None) -> None:
+    """q, scale = e4m3 values and f32 scales of x (of x.T with transpose) in
+    blocks of block_rows (1 or 128) x 128; x is approximately q * scale.
+
+    q is rows x cols of the quantised matrix (torch.float8_e4m3fn or uint8,
+    rows may be padded); scale is [row blocks, column blocks] with any positive
+    strides. torch.empty(column blocks, row blocks).t() is the layout that
+    gemm_block_scaled reads fastest."""
+    d = QuantDesc()
+    d.rows, d.cols = x.shape
+    r, c = (d.cols, d.rows) if transpose else (d.rows, d.cols)
+    d.dtype, d.transpose, d.block_rows = dtype_code(x), int(transpose), block_rows
+    d.ldx = _matrix(x, d.rows, d.cols, "x")
+    d.ldq = _e4m3_matrix(q, r, c, "q")
+    if block_rows in (1, 128):  # anything else is refused below
+        d.scale_row, d.scale_blk = _scales(scale, -(-r // block_rows), -(-c // 128), "scale")
+    d.x, d.q, d.scale = _ptr(x), _ptr(q), _ptr(scale)
+    check(lib.choreo_quantize_block(C.byref(d), _stream_ptr(stream)))
+
+
+def gemm_block_desc(a, scale_a, b, scale_b, c, *, alpha=1.0, beta=0.0, addend=None, bias=None,
+                    relu=False) -> GemmBlockDesc:
+    d = GemmBlockDesc()
+    d.m, d.k = a.shape
+    d.n = b.shape[0]
+    blocks = -(-d.k // 128)
+    d.lda, d.ldb = _e4m3_matrix(a, d.m, d.k, "a"), _e4m3_matrix(b, d.n, d.k, "b")
+    d.scale_a_row, d.scale_a_blk = _scales(scale_a, d.m, blocks, "scale_a")
+    d.block_b = 1 if scale_b.dim() == 2 and scale_b.shape[0] == d.n else 128
+    d.scale_b_row, d.scale_b_blk = _scales(scale_b, -(-d.n // d.block_b), blocks, "scale_b")
+    d.ldc, d.dtype_c = _matrix(c, d.m, d.n, "c"), dtype_code(c)
+    d.a, d.scale_a, d.b, d.scale_b, d.c = map(_ptr, (a, scale_a, b, scale_b, c))
+    d.alpha, d.beta = alpha, beta
+    if addend is not None:
+        d.addend, d.ld_addend = _ptr(addend), _matrix(addend, d.m, d.n, "addend", c)
+    d.bias = _ptr(bias)
+    d.dtype_bias = dtype_code(bias) if bias is not None else F32
+    d.relu = int(relu)
+    return d
+
+
+def gemm_block_scaled_query(d: GemmBlockDesc) -> LaunchConfig:
+    out = LaunchConfig()
+    check(lib.choreo_gemm_block_scaled_query(C.byref(d), C.byref(out)))
+    return out
+
+
+def gemm_block_scaled(a, scale_a, b, scale_b, c, *, alpha=1.0, beta=0.0, addend=None, bias=None, relu=False,
+                      stream=None) -> None:
+    """c = act(alpha * (a * scale_a) @ (b * scale_b).T + beta * addend + bias).
+
+    a is M x K and b N x K in e4m3 (torch.float8_e4m3fn or uint8; rows start on
+    16-byte boundaries), with f32 scales per 1 x 128 block of a and per 1 x 128
+    or 128 x 128 block of b, as quantize_block writes them. addend defaults to
+    c itself."""
+    d = gemm_block_desc(a, scale_a, b, scale_b, c, alpha=alpha, beta=beta, addend=addend, bias=bias, relu=relu)
+    check(lib.choreo_gemm_block_scaled(C.byref(d), _stream_ptr(stream)))
 
 
 def sync_status(stream=None) -> None:

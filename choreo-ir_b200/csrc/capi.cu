@@ -228,13 +228,6 @@ int encode_tmap_im2col(CUtensorMap* map, CUtensorMapDataType dtype, const void* 
 }
 
 // ------------------------------------------------------------------ GEMM planning
-namespace {
-
-bool is_tc_type(int dt) { return dt == CHOREO_DTYPE_F16 || dt == CHOREO_DTYPE_BF16; }
-bool is_float_type(int dt) { return is_tc_type(dt) || dt == CHOREO_DTYPE_F32; }
-int64_t round_up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
-
-// Confirms `p` is memory the current device can read (device, or managed).
 int check_device_ptr(const void* p, const char* name) {
   cudaPointerAttributes attr{};
   cudaError_t e = cudaPointerGetAttributes(&attr, p);
@@ -251,6 +244,8 @@ int check_device_ptr(const void* p, const char* name) {
                 attr.device, dev);
   return CHOREO_OK;
 }
+
+namespace {
 
 int validate_gemm(const choreo_gemm_desc* d) {
   if (d == nullptr) return fail(CHOREO_ERR_INVALID_ARG, "GEMM: null descriptor");
@@ -294,28 +289,6 @@ int validate_gemm(const choreo_gemm_desc* d) {
   if ((rc = check_device_ptr(d->c, "GEMM C"))) return rc;
   if (d->bias && (rc = check_device_ptr(d->bias, "GEMM bias"))) return rc;
   return CHOREO_OK;
-}
-
-// An operand the TMA cannot address directly gets repacked into the workspace.
-struct OperandPlan {
-  bool repack = false;
-  int64_t outer = 0, inner = 0, ld_pad = 0;
-  int64_t bytes = 0, offset = 0;
-};
-
-OperandPlan plan_operand(const void* ptr, int64_t ld, int64_t stride, int64_t batch, int64_t outer,
-                         int64_t inner) {
-  OperandPlan o;
-  o.outer = outer;
-  o.inner = inner;
-  const bool legal = (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0 && (ld * 2) % 16 == 0 &&
-                     (batch == 1 || (stride > 0 && (stride * 2) % 16 == 0));
-  if (!legal) {
-    o.repack = true;
-    o.ld_pad = round_up(inner, 8);
-    o.bytes = round_up(batch * outer * o.ld_pad * 2, 256);
-  }
-  return o;
 }
 
 struct GemmPlan {

@@ -31,6 +31,8 @@ namespace choreo_sm100 {
 // CTA-pair TMA form (bytes counted on the pair leader's barrier).
 template <int BNL, bool PAIR>
 struct ConvLoader {
+  using MapA = CUtensorMap;
+  using MapB = CUtensorMap;
   static constexpr bool kAMn = false;
   static constexpr bool kBMn = false;
   // 128 output pixels starting at pixel m0 (NHW order) for k-block kb = (r, s, channel block).
@@ -151,7 +153,7 @@ template <typename OutT>
 int launch_conv_wide(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const TcParams& kp,
                      int grid, cudaStream_t stream) {
   constexpr int smem = tc_wide_smem_bytes<kConvWideStages>();
-  auto kern = tc_gemm_pair_wide_kernel<kConvWideStages, ConvLoader<128, true>, OutT>;
+  auto kern = tc_gemm_pair_wide_kernel<kConvWideStages, ConvLoader<128, true>, LinearEpi<OutT>>;
   static std::atomic<uint64_t> attr_done{0};
   if (int rc = set_smem_limit_once(kern, smem, attr_done, "cudaFuncSetAttribute(conv wide)")) return rc;
   cudaError_t e;
@@ -165,7 +167,7 @@ int launch_conv_one(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensor
                     int grid, cudaStream_t stream) {
   constexpr int STAGES = conv_stages(BN);
   constexpr int smem = tc_smem_bytes<BN, STAGES>();
-  auto kern = tc_gemm_kernel<BN, STAGES, ConvLoader<BN, false>, OutT>;
+  auto kern = tc_gemm_kernel<BN, STAGES, ConvLoader<BN, false>, LinearEpi<OutT>>;
   static std::atomic<uint64_t> attr_done{0};
   if (int rc = set_smem_limit_once(kern, smem, attr_done, "cudaFuncSetAttribute(conv)")) return rc;
   cudaError_t e;
@@ -179,7 +181,7 @@ int launch_conv_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtenso
                      int grid, cudaStream_t stream) {
   constexpr int STAGES = conv_pair_stages(BN);
   constexpr int smem = tc_pair_smem_bytes<BN, STAGES>();
-  auto kern = tc_gemm_pair_kernel<BN, STAGES, ConvLoader<BN / 2, true>, OutT>;
+  auto kern = tc_gemm_pair_kernel<BN, STAGES, ConvLoader<BN / 2, true>, LinearEpi<OutT>>;
   static std::atomic<uint64_t> attr_done{0};
   if (int rc = set_smem_limit_once(kern, smem, attr_done, "cudaFuncSetAttribute(conv pair)")) return rc;
   cudaError_t e;

@@ -1,0 +1,607 @@
+// gemm_block.cu — C = act(alpha * S + beta * D + bias) for e4m3 operands with
+// an fp32 scale for each block of 128 along K:
+//   S[i,j] = sum_t sa(i,t) sb(j,t) * P_t[i,j],  P_t = A_t B_t^T over block t.
+//
+// The tensor cores sum one block: a k-block of the pipeline is exactly one
+// scale block (128 e4m3 = 128 bytes per row), so each starts a fresh
+// accumulator in TMEM. The epilogue warps read it out, multiply by the two
+// scales and add it to the tile's fp32 sum, which stays in their registers for
+// the whole tile; the next block runs meanwhile in the other accumulator.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <cstring>
+
+#include "internal.h"
+#include "tc_kernel.cuh"
+
+namespace choreo_sm100 {
+
+constexpr int kBlockThreads = 384;  // warpgroup 0: producer, MMA issuer; warpgroups 1 and 2: epilogue
+constexpr int kBlockK = 128;        // e4m3 elements (bytes) per k-block
+
+struct BlockParams : TcParams {
+  const float* sa;
+  int64_t sa_row, sa_blk;
+  const float* sb;
+  int64_t sb_row, sb_blk;
+  const void* d;        // addend
+  int64_t ldd;
+  int32_t d_vec;
+};
+
+template <bool PAIR, int BN>
+struct BlockShape {
+  static constexpr int kBRows = PAIR ? BN / 2 : BN;  // B rows one CTA stages
+  static constexpr uint32_t kAStage = kBM * kBlockK;
+  static constexpr uint32_t kBStage = kBRows * kBlockK;
+  static constexpr int kStages = 6;
+  static constexpr int kSmem = kStages * static_cast<int>(kAStage + kBStage) + kStagingBytes + 1024 +
+                               static_cast<int>(sizeof(TcBarriers<kStages>));
+  // 128 sums a thread and two 32-column reads in flight need more registers
+  // than an even share of the SM's
+  static constexpr bool kMoveRegs = BN == 256;
+  static constexpr int kEpiRegs = 224, kOtherRegs = 56;
+};
+static_assert(BlockShape<true, 256>::kEpiRegs * 256 + BlockShape<true, 256>::kOtherRegs * 128 <= 168 * kBlockThreads,
+              "the warpgroups' shares must fit the registers of the launch");
+
+__device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+// (d0, d1) += (a0, a1) * (s0, s1), one rounding per element.
+__device__ __forceinline__ void fma2_acc(float& d0, float& d1, uint32_t a0, uint32_t a1, uint64_t s) {
+  uint64_t d = pack_f32x2(d0, d1);
+  const uint64_t a = pack_f32x2(__uint_as_float(a0), __uint_as_float(a1));
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(s));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d0), "=f"(d1) : "l"(d));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ void ld_shared_2x64(uint32_t addr, uint64_t& a, uint64_t& b) {
+  asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(a), "=l"(b) : "r"(addr));
+}
+
+// Writes one warp's 32 rows x kCols columns of sums.
+template <int kCols, typename OutT>
+__device__ __forceinline__ void block_output(const float (&acc)[kCols], int n_first, int row0, const BlockParams& p,
+                                             const CUtensorMap* tma_c, uint32_t stage_buf, int lane) {
+  constexpr int E = 128 / static_cast<int>(sizeof(OutT));  // columns per 128-byte staging row
+  constexpr int kCpg = E / 32;
+  const int row = row0 + lane;
+  const bool row_ok = row < p.m;
+  const OutT* drow = static_cast<const OutT*>(p.d) + static_cast<int64_t>(row_ok ? row : 0) * p.ldd;
+  OutT* crow = static_cast<OutT*>(p.c) + static_cast<int64_t>(row_ok ? row : 0) * p.ldc;
+  TcParams pd = p;
+  pd.c_vec_ok = p.d_vec;
+#pragma unroll
+  for (int g = 0; g < kCols / E; ++g) {
+    const int n_base = n_first + g * E;
+    if (n_base >= p.n) break;  // warp-uniform
+    if (p.c_tma) {
+      if (lane == 0) bulk_wait_read_all();  // the warp's previous store has read the buffer
+      __syncwarp();
+    }
+#pragma unroll
+    for (int c = 0; c < kCpg; ++c) {
+      uint32_t r[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(acc[g * E + c * 32 + i]);
+      float v[32];
+      epilogue_values<OutT>(r, v, drow, n_base + c * 32, pd, row_ok, lane);
+      if (p.c_tma) {
+        stage_row_32<OutT>(v, stage_buf + static_cast<uint32_t>(lane) * 128u, lane,
+                           c * (32 * static_cast<int>(sizeof(OutT)) / 16));
+      } else if (row_ok) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (n_base + c * 32 + i < p.n) crow[n_base + c * 32 + i] = from_f32<OutT>(v[i]);
+      }
+    }
+    if (p.c_tma) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_3d(tma_c, stage_buf, n_base, row0, 0);
+        bulk_commit_group();
+      }
+    }
+  }
+}
+
+// BVEC: a scale per row of B (1 x 128 blocks), else one per 128 rows.
+template <bool PAIR, int BN, bool BVEC, typename OutT>
+__device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUtensorMap* tma_b, const CUtensorMap* tma_c,
+                                           const BlockParams& p) {
+  using S = BlockShape<PAIR, BN>;
+  constexpr int STAGES = S::kStages;
+  constexpr int kCols = BN / 2;  // columns of one epilogue warp
+  constexpr uint32_t kTmemCols = 2 * BN;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
+  uint8_t* s_a = smem;
+  uint8_t* s_b = smem + STAGES * S::kAStage;
+  uint8_t* s_stage = s_b + STAGES * S::kBStage;
+  auto* bars = reinterpret_cast<TcBarriers<STAGES>*>(s_stage + kStagingBytes);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? cluster_ctarank() : 0;
+  const bool leader = rank == 0;
+  const int64_t first = PAIR ? blockIdx.x >> 1 : blockIdx.x;
+  const int64_t step = PAIR ? gridDim.x >> 1 : gridDim.x;
+  constexpr int kTileM = PAIR ? 2 * kBM : kBM;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(smem_u32(&bars->full[s]), 1);
+      mbar_init(smem_u32(&bars->empty[s]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&bars->tmem_full[i]), 1);
+      mbar_init(smem_u32(&bars->tmem_empty[i]), (PAIR ? 2 : 1) * kEpiWarps);
+    }
+    mbar_init(smem_u32(&bars->drain), 1);
+    bars->abort = 0;
+    probe_start(p, bars->probe);
+    fence_mbar_init();
+    tma_prefetch_desc(tma_a);
+    tma_prefetch_desc(tma_b);
+    if (p.c_tma) tma_prefetch_desc(tma_c);
+  }
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      tmem_alloc_pair(smem_u32(&bars->tmem_base), kTmemCols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(&bars->tmem_base), kTmemCols);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  if constexpr (PAIR) cluster_sync(); else __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = bars->tmem_base;
+  const WaitCtx wctx{p.status, p.timeout_ns, &bars->abort};
+
+  if (warp < 4) {
+    if constexpr (S::kMoveRegs) regs_dec<S::kOtherRegs>();
+    if (warp == 0 && lane == 0) {
+      // ---------------------------------------------------------- producer
+      griddep_wait();
+      const uint64_t pol_a = l2_policy(p.l2_policy_a);
+      const uint64_t pol_b = l2_policy(p.l2_policy_b);
+      uint32_t stage = 0, phase = 0, issued = 0;
+      bool ok = true;
+      for (int64_t t = first; t < p.num_tiles && ok; t += step) {
+        int b, mb, nb;
+        tile_coords(t, p, b, mb, nb);
+        const int m0 = mb * kTileM + static_cast<int>(rank) * kBM;
+        const int n0 = nb * BN + static_cast<int>(rank) * S::kBRows;
+        for (int kb = 0; kb < p.num_k_blocks; ++kb) {
+          if (!mbar_wait(smem_u32(&bars->empty[stage]), phase ^ 1, wctx, kStatusTimeoutProducer)) {
+            ok = false;
+            break;
+          }
+          const uint32_t fb = smem_u32(&bars->full[stage]);
+          if (leader) mbar_arrive_expect_tx(fb, (PAIR ? 2 : 1) * (S::kAStage + S::kBStage));
+          const uint32_t bar = PAIR ? mapa_shared(fb, 0) : fb;
+          load3<PAIR>(smem_u32(s_a + stage * S::kAStage), tma_a, bar, kb * kBlockK, m0, 0, pol_a);
+          load3<PAIR>(smem_u32(s_b + stage * S::kBStage), tma_b, bar, kb * kBlockK, n0, 0, pol_b);
+          ++issued;
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+      griddep_launch_dependents();
+      if (!ok) {
+        if (leader) {
+          const uint32_t inflight = issued < STAGES ? issued : STAGES;
+          uint32_t s = stage, ph = phase;
+          for (uint32_t i = 0; i < inflight; ++i) {
+            if (s == 0) { s = STAGES - 1; ph ^= 1; } else { --s; }
+            mbar_wait(smem_u32(&bars->full[s]), ph, wctx, kStatusTimeoutDrain, false);
+          }
+        } else {
+          // The peer's loads count on the leader's barriers: give them time to land.
+          const uint64_t t0 = globaltimer_ns();
+          while (globaltimer_ns() - t0 < 200000ull) {
+          }
+        }
+      }
+    } else if (warp == 1 && leader && lane == 0) {
+      // ---------------------------------------------------------- MMA issuer
+      const uint32_t idesc = idesc_e4m3(kTileM, BN);
+      uint32_t stage = 0, phase = 0, blocks = 0;
+      bool ok = true;
+      for (int64_t t = first; t < p.num_tiles && ok; t += step) {
+        for (int kb = 0; kb < p.num_k_blocks; ++kb, ++blocks) {
+          const uint32_t buf = blocks & 1;
+          if (!mbar_wait(smem_u32(&bars->tmem_empty[buf]), ((blocks >> 1) & 1) ^ 1, wctx, kStatusTimeoutMma) ||
+              !mbar_wait(smem_u32(&bars->full[stage]), phase, wctx, kStatusTimeoutMma)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(s_a + stage * S::kAStage);
+          const uint32_t b0 = smem_u32(s_b + stage * S::kBStage);
+#pragma unroll
+          for (int k = 0; k < kBlockK / 32; ++k) {
+            const uint64_t ad = smem_desc_sw128(a0 + k * 32, 16, 1024);
+            const uint64_t bd = smem_desc_sw128(b0 + k * 32, 16, 1024);
+            if constexpr (PAIR)
+              umma_f8_pair(tmem_base + buf * BN, ad, bd, idesc, k != 0 ? 1u : 0u);
+            else
+              umma_f8(tmem_base + buf * BN, ad, bd, idesc, k != 0 ? 1u : 0u);
+          }
+          const uint32_t eb = smem_u32(&bars->empty[stage]);
+          const uint32_t tf = smem_u32(&bars->tmem_full[buf]);
+          if constexpr (PAIR) {
+            umma_commit_pair(eb);
+            umma_commit_pair(mapa_shared(eb, 1));
+            umma_commit_pair(tf);
+            umma_commit_pair(mapa_shared(tf, 1));
+          } else {
+            umma_commit(eb);
+            umma_commit(tf);
+          }
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+      if constexpr (PAIR) umma_commit_pair(smem_u32(&bars->drain)); else umma_commit(smem_u32(&bars->drain));
+      mbar_wait(smem_u32(&bars->drain), 0, wctx, kStatusTimeoutDrain, false);
+    }
+  } else {
+    if constexpr (S::kMoveRegs) regs_inc<S::kEpiRegs>();
+    // ------------------------------------------------------------ epilogue
+    const int quarter = warp & 3;
+    const int col_half = (warp - 4) >> 2;
+    const uint32_t stage_buf = smem_u32(s_stage) + static_cast<uint32_t>(warp - 4) * 4096u;
+    griddep_wait();
+    uint32_t blocks = 0;
+    bool ok = true;
+    for (int64_t t = first; t < p.num_tiles && ok; t += step) {
+      int b, mb, nb;
+      tile_coords(t, p, b, mb, nb);
+      const int row0 = mb * kTileM + static_cast<int>(rank) * kBM + quarter * 32;
+      const int n_first = nb * BN + col_half * kCols;
+      const bool active = row0 < p.m && n_first < p.n;
+      const int row = min(row0 + lane, p.m - 1);
+      const float* sa = p.sa + static_cast<int64_t>(row) * p.sa_row;
+      // BVEC: lane l holds the scales of columns n_first + 32 c + l
+      const float* sb[BVEC ? kCols / 32 : 1];
+      if constexpr (BVEC) {
+#pragma unroll
+        for (int c = 0; c < kCols / 32; ++c)
+          sb[c] = p.sb + static_cast<int64_t>(min(n_first + 32 * c + lane, p.n - 1)) * p.sb_row;
+      } else {
+        sb[0] = p.sb + static_cast<int64_t>(min(n_first, p.n - 1) / 128) * p.sb_row;
+      }
+      float acc[kCols];
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
+      float next_a = __ldg(sa);
+      float next_b[BVEC ? kCols / 32 : 1];
+#pragma unroll
+      for (int c = 0; c < (BVEC ? kCols / 32 : 1); ++c) next_b[c] = __ldg(sb[c]);
+      if constexpr (BVEC) {
+        if (lane == 0) bulk_wait_read_all();  // the previous tile's stores have read the buffer
+        __syncwarp();
+      }
+#pragma unroll 1
+      for (int kb = 0; kb < p.num_k_blocks; ++kb, ++blocks) {
+        const uint32_t buf = blocks & 1;
+        const float cur_a = next_a;
+        float s = 0.f;
+        uint32_t sbuf = 0;
+        if constexpr (BVEC) {
+          // the block's column scales, read back below as broadcasts
+          sbuf = stage_buf + (kb & 1) * 512u;
+#pragma unroll
+          for (int c = 0; c < kCols / 32; ++c) st_shared_f32(sbuf + static_cast<uint32_t>(c * 32 + lane) * 4u, next_b[c]);
+          __syncwarp();
+        } else {
+          s = cur_a * next_b[0];
+        }
+        if (kb + 1 < p.num_k_blocks) {
+          next_a = __ldg(sa + static_cast<int64_t>(kb + 1) * p.sa_blk);
+#pragma unroll
+          for (int c = 0; c < (BVEC ? kCols / 32 : 1); ++c)
+            next_b[c] = __ldg(sb[c] + static_cast<int64_t>(kb + 1) * p.sb_blk);
+        }
+        const bool ready = mbar_wait(smem_u32(&bars->tmem_full[buf]), (blocks >> 1) & 1, wctx, kStatusTimeoutEpilogue);
+        if (!__all_sync(0xffffffffu, ready)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t taddr =
+            tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN + col_half * kCols;
+        auto release = [&] {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            const uint32_t eb = smem_u32(&bars->tmem_empty[buf]);
+            if (leader)
+              mbar_arrive(eb);
+            else
+              mbar_arrive_cluster(mapa_shared(eb, 0));
+          }
+        };
+        if (!active) {
+          release();
+          continue;
+        }
+        uint32_t r[2][32];
+        tmem_ld_32x32b_x32(taddr, r[0]);
+        tmem_wait_ld(r[0]);
+#pragma unroll
+        for (int c = 0; c < kCols / 32; ++c) {
+          if (c + 1 < kCols / 32) tmem_ld_32x32b_x32(taddr + (c + 1) * 32, r[(c + 1) & 1]);
+          else release();
+          if constexpr (BVEC) {
+            const uint64_t a2 = pack_f32x2(cur_a, cur_a);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              uint64_t b0, b1;
+              ld_shared_2x64(sbuf + static_cast<uint32_t>(c * 32 + 4 * j) * 4u, b0, b1);
+              fma2_acc(acc[c * 32 + 4 * j], acc[c * 32 + 4 * j + 1], r[c & 1][4 * j], r[c & 1][4 * j + 1], mul2(a2, b0));
+              fma2_acc(acc[c * 32 + 4 * j + 2], acc[c * 32 + 4 * j + 3], r[c & 1][4 * j + 2], r[c & 1][4 * j + 3],
+                       mul2(a2, b1));
+            }
+          } else {
+            const uint64_t s2 = pack_f32x2(s, s);
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              fma2_acc(acc[c * 32 + 2 * j], acc[c * 32 + 2 * j + 1], r[c & 1][2 * j], r[c & 1][2 * j + 1], s2);
+          }
+          if (c + 1 < kCols / 32) tmem_wait_ld(r[(c + 1) & 1]);
+        }
+      }
+      if (ok && active) block_output<kCols, OutT>(acc, n_first, row0, p, tma_c, stage_buf, lane);
+    }
+    if (lane == 0) bulk_wait_read_all();
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  if constexpr (PAIR) cluster_sync(); else __syncthreads();
+  probe_end(p, bars->probe);
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (PAIR) tmem_dealloc_pair(tmem_base, kTmemCols); else tmem_dealloc(tmem_base, kTmemCols);
+  }
+}
+
+template <int BN, bool BVEC, typename OutT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBlockThreads, 1)
+    block_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
+                      const __grid_constant__ CUtensorMap tma_c, const BlockParams p) {
+  block_body<true, BN, BVEC, OutT>(&tma_a, &tma_b, &tma_c, p);
+}
+template <int BN, bool BVEC, typename OutT>
+__global__ void __launch_bounds__(kBlockThreads, 1)
+    block_single_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
+                        const __grid_constant__ CUtensorMap tma_c, const BlockParams p) {
+  block_body<false, BN, BVEC, OutT>(&tma_a, &tma_b, &tma_c, p);
+}
+
+}  // namespace choreo_sm100
+
+namespace choreo_impl {
+using namespace choreo_sm100;
+
+namespace {
+
+struct BlockConfig {
+  bool pair;
+  int bn;
+};
+
+BlockConfig select_block_config(int64_t m, int64_t n) {
+  const int sms = current_sm_count();
+  const int64_t pairs = ((m + 255) / 256) * ((n + 255) / 256);
+  return pairs * 2 >= sms ? BlockConfig{true, 256} : BlockConfig{false, 128};
+}
+
+template <typename Kern>
+int launch_block(Kern kern, int smem, bool move_regs, std::atomic<uint64_t>& attr_done, const CUtensorMap& ta,
+                 const CUtensorMap& tb, const CUtensorMap& tc, const BlockParams& kp, int grid, cudaStream_t s) {
+  if (int rc = set_smem_limit_once(kern, smem, attr_done, "cudaFuncSetAttribute(block-scaled GEMM)")) return rc;
+  if (move_regs) {
+    // The epilogue's larger share comes out of the launch's registers: it must be there.
+    static thread_local const void* checked = nullptr;
+    if (checked != reinterpret_cast<const void*>(kern)) {
+      cudaFuncAttributes fa{};
+      const cudaError_t e = cudaFuncGetAttributes(&fa, kern);
+      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncGetAttributes(block-scaled GEMM)");
+      if (fa.numRegs < 168)
+        return fail(CHOREO_ERR_UNSUPPORTED, "block-scaled GEMM: built with %d registers per thread, needs 168", fa.numRegs);
+      checked = reinterpret_cast<const void*>(kern);
+    }
+  }
+  const cudaError_t e = launch_pdl(kern, dim3(grid), dim3(kBlockThreads), smem, s, ta, tb, tc, kp);
+  return e == cudaSuccess ? CHOREO_OK : cuda_fail(e, "block-scaled GEMM launch");
+}
+
+template <bool BVEC, typename OutT>
+int dispatch_block(const BlockConfig& c, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc,
+                   const BlockParams& kp, int grid, cudaStream_t s) {
+  if (c.pair) {
+    using S = BlockShape<true, 256>;
+    static std::atomic<uint64_t> done{0};
+    return launch_block(block_pair_kernel<256, BVEC, OutT>, S::kSmem, S::kMoveRegs, done, ta, tb, tc, kp, grid, s);
+  }
+  using S = BlockShape<false, 128>;
+  static std::atomic<uint64_t> done{0};
+  return launch_block(block_single_kernel<128, BVEC, OutT>, S::kSmem, S::kMoveRegs, done, ta, tb, tc, kp, grid, s);
+}
+
+int encode_e4m3(CUtensorMap* map, const void* p, int64_t rows, int64_t k, int64_t ld, uint32_t box_rows) {
+  const uint64_t dims[3] = {static_cast<uint64_t>(k), static_cast<uint64_t>(rows), 1};
+  const uint64_t strides[2] = {static_cast<uint64_t>(ld), static_cast<uint64_t>(rows) * static_cast<uint64_t>(ld)};
+  const uint32_t box[3] = {kBlockK, box_rows, 1};
+  return encode_tmap(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, p, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int validate_block(const choreo_gemm_block_desc* d) {
+  const char* what = "block-scaled GEMM";
+  if (d == nullptr) return fail(CHOREO_ERR_INVALID_ARG, "%s: null descriptor", what);
+  if (d->m <= 0 || d->n <= 0 || d->k <= 0)
+    return fail(CHOREO_ERR_INVALID_ARG, "%s: Invalid matrix dimensions: M=%lld, N=%lld, K=%lld", what, (long long)d->m,
+                (long long)d->n, (long long)d->k);
+  if (d->m > INT32_MAX / 2 || d->n > INT32_MAX / 2 || d->k > INT32_MAX / 2)
+    return fail(CHOREO_ERR_UNSUPPORTED, "%s: dimensions above 2^30-1 are not supported", what);
+  if (d->a == nullptr || d->b == nullptr) return fail(CHOREO_ERR_INVALID_ARG, "%s: an operand has null data pointer", what);
+  if (d->scale_a == nullptr || d->scale_b == nullptr)
+    return fail(CHOREO_ERR_INVALID_ARG, "%s: a scale has null data pointer", what);
+  if (d->c == nullptr) return fail(CHOREO_ERR_INVALID_ARG, "%s: Output tensor C has null data pointer", what);
+  if (!is_float_type(d->dtype_c)) return fail(CHOREO_ERR_UNSUPPORTED, "%s: unsupported output dtype %d", what, d->dtype_c);
+  if (d->block_b != 1 && d->block_b != 128)
+    return fail(CHOREO_ERR_UNSUPPORTED, "%s: block_b %d is neither 1 nor 128", what, d->block_b);
+  if (d->lda < d->k || d->ldb < d->k)
+    return fail(CHOREO_ERR_INVALID_ARG, "%s: lda=%lld or ldb=%lld smaller than K=%lld", what, (long long)d->lda,
+                (long long)d->ldb, (long long)d->k);
+  if (d->lda % 16 != 0 || d->ldb % 16 != 0 || (reinterpret_cast<uintptr_t>(d->a) & 15u) != 0 ||
+      (reinterpret_cast<uintptr_t>(d->b) & 15u) != 0)
+    return fail(CHOREO_ERR_INVALID_ARG,
+                "%s: A, B and their leading dimensions must be multiples of 16 bytes (lda=%lld, ldb=%lld)", what,
+                (long long)d->lda, (long long)d->ldb);
+  if (d->ldc < d->n)
+    return fail(CHOREO_ERR_INVALID_ARG, "%s: ldc=%lld smaller than N=%lld", what, (long long)d->ldc, (long long)d->n);
+  if (d->scale_a_row < 0 || d->scale_a_blk < 0 || d->scale_b_row < 0 || d->scale_b_blk < 0)
+    return fail(CHOREO_ERR_INVALID_ARG, "%s: negative scale stride", what);
+  if (d->addend && d->ld_addend < d->n)
+    return fail(CHOREO_ERR_INVALID_ARG, "%s: ld_addend=%lld smaller than N=%lld", what, (long long)d->ld_addend,
+                (long long)d->n);
+  if (d->bias && !is_float_type(d->dtype_bias))
+    return fail(CHOREO_ERR_UNSUPPORTED, "%s: unsupported bias dtype %d", what, d->dtype_bias);
+  const struct {
+    const void* p;
+    const char* name;
+  } ptrs[] = {{d->a, "block-scaled GEMM A"},           {d->b, "block-scaled GEMM B"},
+              {d->scale_a, "block-scaled GEMM scale A"}, {d->scale_b, "block-scaled GEMM scale B"},
+              {d->c, "block-scaled GEMM C"},           {d->beta != 0.f ? d->addend : nullptr, "block-scaled GEMM addend"},
+              {d->bias, "block-scaled GEMM bias"}};
+  for (const auto& q : ptrs)
+    if (q.p)
+      if (int rc = check_device_ptr(q.p, q.name)) return rc;
+  return CHOREO_OK;
+}
+
+int64_t block_tiles(const choreo_gemm_block_desc& d, const BlockConfig& c) {
+  const int64_t rows = c.pair ? 256 : 128;
+  return ((d.m + rows - 1) / rows) * ((d.n + c.bn - 1) / c.bn);
+}
+int block_grid(int64_t tiles, const BlockConfig& c) {
+  const int sms = current_sm_count();
+  return static_cast<int>(c.pair ? 2 * std::min<int64_t>(tiles, sms / 2) : std::min<int64_t>(tiles, sms));
+}
+
+}  // namespace
+}  // namespace choreo_impl
+
+using namespace choreo_impl;
+
+extern "C" {
+
+int choreo_gemm_block_scaled_query(const choreo_gemm_block_desc* d, choreo_launch_config* out) {
+  int rc = validate_block(d);
+  if (rc) return rc;
+  if (out == nullptr) return fail(CHOREO_ERR_INVALID_ARG, "block-scaled GEMM query: null output");
+  std::memset(out, 0, sizeof(*out));
+  const BlockConfig c = select_block_config(d->m, d->n);
+  out->kernel = 5;
+  out->tile_m = c.pair ? 256 : 128;
+  out->tile_n = c.bn;
+  out->tile_k = kBlockK;
+  out->stages = BlockShape<true, 256>::kStages;
+  out->cluster_m = c.pair ? 2 : 1;
+  out->tiles = block_tiles(*d, c);
+  out->grid_x = block_grid(out->tiles, c);
+  out->grid_y = out->grid_z = 1;
+  out->block_x = kBlockThreads;
+  out->smem_bytes = c.pair ? BlockShape<true, 256>::kSmem : BlockShape<false, 128>::kSmem;
+  out->tmem_cols = 2 * c.bn;
+  out->split_k = 1;
+  return ok();
+}
+
+int choreo_gemm_block_scaled(const choreo_gemm_block_desc* d, void* stream) {
+  int rc = validate_block(d);
+  if (rc) return rc;
+  const BlockConfig c = select_block_config(d->m, d->n);
+  CUtensorMap ta, tb, tc;
+  if ((rc = encode_e4m3(&ta, d->a, d->m, d->k, d->lda, 128))) return rc;
+  if ((rc = encode_e4m3(&tb, d->b, d->n, d->k, d->ldb, 128))) return rc;
+  BlockParams kp;
+  std::memset(&kp, 0, sizeof(kp));
+  kp.m = static_cast<int32_t>(d->m);
+  kp.n = static_cast<int32_t>(d->n);
+  kp.num_k_blocks = static_cast<int32_t>((d->k + kBlockK - 1) / kBlockK);
+  const int rows = c.pair ? 256 : 128;
+  kp.num_m_blocks = static_cast<int32_t>((d->m + rows - 1) / rows);
+  kp.num_n_blocks = static_cast<int32_t>((d->n + c.bn - 1) / c.bn);
+  kp.batch = 1;
+  kp.num_tiles = block_tiles(*d, c);
+  const L2Plan l2 = l2_plan();
+  kp.group_m = group_tiles(l2, rows, kp.num_m_blocks);
+  kp.l2_policy_a = l2.policy_a;
+  kp.l2_policy_b = l2.policy_b;
+  kp.c = d->c;
+  kp.ldc = d->ldc;
+  kp.alpha = d->alpha;
+  kp.beta = d->beta;
+  kp.bias = d->bias;
+  kp.dtype_bias = d->dtype_bias;
+  kp.relu = d->relu;
+  kp.sa = d->scale_a;
+  kp.sa_row = d->scale_a_row;
+  kp.sa_blk = d->scale_a_blk;
+  kp.sb = d->scale_b;
+  kp.sb_row = d->scale_b_row;
+  kp.sb_blk = d->scale_b_blk;
+  kp.d = d->addend ? d->addend : d->c;
+  kp.ldd = d->addend ? d->ld_addend : d->ldc;
+  const int eb = dtype_bytes(d->dtype_c);
+  kp.d_vec = ((reinterpret_cast<uintptr_t>(kp.d) | static_cast<uintptr_t>(kp.ldd * eb)) & 15u) == 0;
+  std::memset(&tc, 0, sizeof(tc));
+  kp.c_vec_ok = kp.c_tma = ((reinterpret_cast<uintptr_t>(d->c) | static_cast<uintptr_t>(d->ldc * eb)) & 15u) == 0;
+  if (kp.c_tma) {
+    const uint64_t dims[3] = {static_cast<uint64_t>(d->n), static_cast<uint64_t>(d->m), 1};
+    const uint64_t strides[2] = {static_cast<uint64_t>(d->ldc) * eb, static_cast<uint64_t>(d->m) * d->ldc * eb};
+    const uint32_t box[3] = {static_cast<uint32_t>(128 / eb), 32, 1};
+    const CUtensorMapDataType dt = d->dtype_c == CHOREO_DTYPE_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : d->dtype_c == CHOREO_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    if ((rc = encode_tmap(&tc, dt, 3, d->c, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
+  }
+  kp.status = status_word();
+  kp.timeout_ns = wait_timeout_ns();
+  kp.clock_probe = clock_probe();
+  if (kp.status == nullptr) return CHOREO_ERR_CUDA;
+  const int grid = block_grid(kp.num_tiles, c);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool vec = d->block_b == 1;
+  switch (d->dtype_c) {
+    case CHOREO_DTYPE_F16:
+      rc = vec ? dispatch_block<true, __half>(c, ta, tb, tc, kp, grid, s)
+               : dispatch_block<false, __half>(c, ta, tb, tc, kp, grid, s);
+      break;
+    case CHOREO_DTYPE_BF16:
+      rc = vec ? dispatch_block<true, __nv_bfloat16>(c, ta, tb, tc, kp, grid, s)
+               : dispatch_block<false, __nv_bfloat16>(c, ta, tb, tc, kp, grid, s);
+      break;
+    default:
+      rc = vec ? dispatch_block<true, float>(c, ta, tb, tc, kp, grid, s)
+               : dispatch_block<false, float>(c, ta, tb, tc, kp, grid, s);
+  }
+  return rc ? rc : ok();
+}
+
+}  // extern "C"

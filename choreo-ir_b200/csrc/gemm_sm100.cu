@@ -21,20 +21,12 @@
 
 namespace choreo_sm100 {
 
-// 3-D tiled load through the single-CTA or the CTA-pair form.
-template <bool PAIR>
-__device__ __forceinline__ void load3(uint32_t dst, const CUtensorMap* map, uint32_t bar, int32_t c0, int32_t c1,
-                                      int32_t c2, uint64_t pol) {
-  if constexpr (PAIR)
-    tma_load_3d_pair(dst, map, bar, c0, c1, c2, pol);
-  else
-    tma_load_3d(dst, map, bar, c0, c1, c2, pol);
-}
-
 // BNL = B columns one CTA stages per k-block (the tile's N for a single CTA,
 // half of it for a CTA pair).
 template <bool A_MN, bool B_MN, int BNL, bool PAIR>
 struct GemmLoader {
+  using MapA = CUtensorMap;
+  using MapB = CUtensorMap;
   static constexpr bool kAMn = A_MN;
   static constexpr bool kBMn = B_MN;
   // With a K split (p.split_kb > 0) the batch index b selects k-blocks
@@ -111,16 +103,12 @@ static_assert(kThreads == kTcThreads, "launch width and reported block size must
 
 namespace {
 
-constexpr int stages_for(int bn) { return bn == 256 ? 4 : (bn == 128 ? 6 : 8); }
-constexpr int pair_stages_for(int bn) { return bn == 256 ? 6 : 8; }
-constexpr int kWideStages = 4;
-
 template <int BN, bool A_MN, bool B_MN, typename OutT>
 int launch_one(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const TcParams& kp, int grid,
                cudaStream_t stream) {
   constexpr int STAGES = stages_for(BN);
   constexpr int smem = tc_smem_bytes<BN, STAGES>();
-  auto kern = tc_gemm_kernel<BN, STAGES, GemmLoader<A_MN, B_MN, BN, false>, OutT>;
+  auto kern = tc_gemm_kernel<BN, STAGES, GemmLoader<A_MN, B_MN, BN, false>, LinearEpi<OutT>>;
   static std::atomic<uint64_t> attr_done{0};
   if (int rc = set_smem_limit_once(kern, smem, attr_done, "cudaFuncSetAttribute(gemm)")) return rc;
   cudaError_t e;
@@ -134,7 +122,7 @@ int launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap&
                 cudaStream_t stream) {
   constexpr int STAGES = pair_stages_for(BN);
   constexpr int smem = tc_pair_smem_bytes<BN, STAGES>();
-  auto kern = tc_gemm_pair_kernel<BN, STAGES, GemmLoader<A_MN, B_MN, BN / 2, true>, OutT>;
+  auto kern = tc_gemm_pair_kernel<BN, STAGES, GemmLoader<A_MN, B_MN, BN / 2, true>, LinearEpi<OutT>>;
   static std::atomic<uint64_t> attr_done{0};
   if (int rc = set_smem_limit_once(kern, smem, attr_done, "cudaFuncSetAttribute(gemm pair)")) return rc;
   cudaError_t e;
@@ -147,7 +135,7 @@ template <bool A_MN, bool B_MN, typename OutT>
 int launch_wide(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const TcParams& kp,
                 int grid, cudaStream_t stream) {
   constexpr int smem = tc_wide_smem_bytes<kWideStages>();
-  auto kern = tc_gemm_pair_wide_kernel<kWideStages, GemmLoader<A_MN, B_MN, 128, true>, OutT>;
+  auto kern = tc_gemm_pair_wide_kernel<kWideStages, GemmLoader<A_MN, B_MN, 128, true>, LinearEpi<OutT>>;
   static std::atomic<uint64_t> attr_done{0};
   if (int rc = set_smem_limit_once(kern, smem, attr_done, "cudaFuncSetAttribute(gemm wide)")) return rc;
   cudaError_t e;
@@ -227,7 +215,7 @@ TcConfig make_config(bool pair, bool wide, int bn) {
 }  // namespace
 
 TilePlan plan_tiles(int64_t m, int64_t n, int64_t k_blocks, int64_t batch, int sm_count, bool allow_split,
-                    int out_bytes) {
+                    int out_bytes, unsigned tiles_built) {
   // Candidates: wide CTA pairs (512 x 256 tiles on 2 SMs), CTA pairs
   // (256 x BN) and single CTAs (128 x BN). A tile puts rows_per_sm x BN
   // outputs on each SM, `area` = rows_per_sm * BN / (128 * 256) slabs. One
@@ -263,7 +251,9 @@ TilePlan plan_tiles(int64_t m, int64_t n, int64_t k_blocks, int64_t batch, int s
   const int64_t want_split = tu.t.split_k;
   TilePlan best{};
   best.est_us = 1e300;
-  for (const Cand& cd : cands) {
+  for (int ci = 0; ci < 6; ++ci) {
+    const Cand& cd = cands[ci];
+    if ((tiles_built >> ci & 1u) == 0) continue;
     if (force && std::strcmp(force, cd.name) != 0) continue;
     const int64_t rows = cd.wide ? 4 * kBM : (cd.pair ? 2 * kBM : kBM);
     const int64_t rows_per_sm = cd.wide ? 2 * kBM : kBM;

@@ -79,6 +79,9 @@ struct Tuning {
 };
 Tuning tuning();
 
+// Confirms `p` is memory the current device can read (device, or managed).
+int check_device_ptr(const void* p, const char* name);
+
 // L2 eviction policy codes handed to the kernels (A operand, B operand) and
 // the tile rasterisation group: defaults, or the tuning overrides
 // (choreo_tuning::l2_policy_a/b, group_m).
@@ -115,13 +118,16 @@ inline int tile_rows_of(const TcConfig& c) { return c.wide ? 512 : (c.pair ? 256
 TcConfig select_tile_config(int64_t m, int64_t n, int64_t k_blocks, int64_t batch, int sm_count);
 // The tile shape and, with allow_split (batch 1), the number of K splits with
 // the lowest estimated time; out_bytes is the size of one output element.
+// tiles_built: which tile shapes the caller's kernel is built for (kTile* bits).
+constexpr unsigned kTileWide256 = 1u << 0, kTilePair256 = 1u << 1, kTileSingle256 = 1u << 2, kTilePair128 = 1u << 3,
+                   kTileSingle128 = 1u << 4, kTileSingle64 = 1u << 5, kAllTiles = (1u << 6) - 1;
 struct TilePlan {
   TcConfig cfg{};
   int64_t split = 1;
   double est_us = 0;
 };
 TilePlan plan_tiles(int64_t m, int64_t n, int64_t k_blocks, int64_t batch, int sm_count, bool allow_split,
-                    int out_bytes);
+                    int out_bytes, unsigned tiles_built = kAllTiles);
 
 // A GEMM with every operand already TMA-legal (16-byte aligned base, ld and
 // batch stride), in the orientation it is stored.
@@ -165,6 +171,31 @@ int launch_relu(int dtype, const void* in, void* out, int64_t n, cudaStream_t s)
 int launch_add(int dtype, const void* a, const void* b, void* out, int64_t n, cudaStream_t s);
 int launch_fill(int dtype, void* dst, double v, int64_t n, cudaStream_t s);
 int launch_convert(int dsrc, const void* src, int ddst, void* dst, int64_t n, cudaStream_t s);
+
+inline bool is_tc_type(int dt) { return dt == CHOREO_DTYPE_F16 || dt == CHOREO_DTYPE_BF16; }
+inline bool is_float_type(int dt) { return is_tc_type(dt) || dt == CHOREO_DTYPE_F32; }
+inline int64_t round_up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
+
+// An operand the TMA cannot address directly gets repacked into the workspace.
+struct OperandPlan {
+  bool repack = false;
+  int64_t outer = 0, inner = 0, ld_pad = 0;
+  int64_t bytes = 0, offset = 0;
+};
+inline OperandPlan plan_operand(const void* ptr, int64_t ld, int64_t stride, int64_t batch, int64_t outer,
+                                int64_t inner) {
+  OperandPlan o;
+  o.outer = outer;
+  o.inner = inner;
+  const bool legal = (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0 && (ld * 2) % 16 == 0 &&
+                     (batch == 1 || (stride > 0 && (stride * 2) % 16 == 0));
+  if (!legal) {
+    o.repack = true;
+    o.ld_pad = round_up(inner, 8);
+    o.bytes = round_up(batch * outer * o.ld_pad * 2, 256);
+  }
+  return o;
+}
 
 inline int dtype_bytes(int dt) {
   switch (dt) {

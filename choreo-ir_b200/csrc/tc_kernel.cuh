@@ -37,6 +37,12 @@ constexpr int kEpiWarps = 8;
 // Epilogue staging: one 4 KB buffer (32 rows x 128 bytes) per epilogue warp.
 constexpr int kStagingBytes = kEpiWarps * 4096;
 
+// Pipeline depth of each tile shape: what fits in shared memory beside the
+// epilogue staging.
+constexpr int stages_for(int bn) { return bn == 256 ? 4 : (bn == 128 ? 6 : 8); }
+constexpr int pair_stages_for(int bn) { return bn == 256 ? 6 : 8; }
+constexpr int kWideStages = 4;
+
 // Everything the kernel needs besides the two tensor maps.
 struct TcParams {
   int32_t m, n;            // output rows / columns (per batch item)
@@ -492,6 +498,53 @@ __device__ __forceinline__ void epilogue_warp(uint32_t taddr, int n_first, int r
   }
 }
 
+// 3-D tiled load through the single-CTA or the CTA-pair form.
+template <bool PAIR>
+__device__ __forceinline__ void load3(uint32_t dst, const CUtensorMap* map, uint32_t bar, int32_t c0, int32_t c1,
+                                      int32_t c2, uint64_t pol) {
+  if constexpr (PAIR)
+    tma_load_3d_pair(dst, map, bar, c0, c1, c2, pol);
+  else
+    tma_load_3d(dst, map, bar, c0, c1, c2, pol);
+}
+
+// Two tensor maps passed as one kernel parameter, for kernels whose loader or
+// epilogue chooses between two matrices.
+struct alignas(64) TwoMaps {
+  CUtensorMap m[2];
+};
+__device__ __forceinline__ void tma_prefetch_desc(const TwoMaps* maps) {
+  tma_prefetch_desc(&maps->m[0]);
+  tma_prefetch_desc(&maps->m[1]);
+}
+
+// Epilogue contract (Epi of the kernels below):
+//   MapC, Params               what the kernel is handed for the outputs; Params is TcParams or derived from it
+//   Pre<BN>, prefetch<BN>(...) values loaded before the wait for the accumulator
+//   run<BN>(tacc, nb, col_half, row0, b, p, maps, stage_buf, lane, pre, release)
+// called by the two warps of a TMEM lane quarter (col_half 0 and 1) for the 32
+// accumulator rows row0 .. row0 + 31 and the BN columns of N tile nb at tacc.
+//
+// LinearEpi: C = act(alpha * acc + beta * C + bias), each warp half the columns.
+template <typename OutT>
+struct LinearEpi {
+  using MapC = CUtensorMap;
+  using Params = TcParams;
+  template <int BN>
+  using Pre = BiasRegs<BN / 2>;
+  template <int BN>
+  __device__ __forceinline__ static void prefetch(Pre<BN>& br, int nb, int col_half, const TcParams& p, int lane) {
+    bias_prefetch(br, nb * BN + col_half * (BN / 2), p, lane);
+  }
+  template <int BN, typename Release>
+  __device__ __forceinline__ static void run(uint32_t tacc, int nb, int col_half, int row0, int b, const TcParams& p,
+                                             const CUtensorMap* tma_c, uint32_t stage_buf, int lane,
+                                             const Pre<BN>& br, Release&& release) {
+    epilogue_warp<BN / 2, OutT>(tacc + col_half * (BN / 2), nb * BN + col_half * (BN / 2), row0, b, p, tma_c, stage_buf,
+                                lane, br, release);
+  }
+};
+
 // Shared-memory bookkeeping beyond the stage ring.
 template <int STAGES>
 struct alignas(8) TcBarriers {
@@ -512,8 +565,9 @@ constexpr int tc_smem_bytes() {
 }
 
 // Loader contract:
+//   MapA, MapB                                 the operands' tensor maps (CUtensorMap, or two of them)
 //   static constexpr bool kAMn, kBMn;          operand majorness in shared memory
-//   __device__ static void issue(const CUtensorMap* ta, const CUtensorMap* tb, const TcParams&,
+//   __device__ static void issue(const MapA* ta, const MapB* tb, const TcParams&,
 //                                int b, int m0, int n0, int kb, uint32_t dst_a, uint32_t dst_b,
 //                                uint32_t bar, uint64_t pol_a, uint64_t pol_b);
 // loads this CTA's A rows [m0, m0 + 128) and B columns [n0, n0 + B width) for
@@ -522,10 +576,11 @@ constexpr int tc_smem_bytes() {
 //   struct WideCursor;  static WideCursor wide_cursor(const TcParams&, int b, int m0, int n0);
 //   static void issue_wide(ta, tb, p, WideCursor&, int kb, dst_a, dst_b, bar, pol_a, pol_b);
 // called for k-blocks 0, 1, ... of one tile in order (this CTA's 256 A rows).
-template <int BN, int STAGES, class Loader, typename OutT>
+template <int BN, int STAGES, class Loader, class Epi>
 __global__ void __launch_bounds__(kThreads, 1)
-    tc_gemm_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
-                   const __grid_constant__ CUtensorMap tma_c, const TcParams p) {
+    tc_gemm_kernel(const __grid_constant__ typename Loader::MapA tma_a,
+                   const __grid_constant__ typename Loader::MapB tma_b,
+                   const __grid_constant__ typename Epi::MapC tma_c, const typename Epi::Params p) {
   constexpr uint32_t kAStage = kBM * kBK * 2;
   constexpr uint32_t kBStage = BN * kBK * 2;
   constexpr uint32_t kStageBytes = kAStage + kBStage;
@@ -658,22 +713,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t tph = (local >> 1) & 1;
       int b, mb, nb;
       tile_coords(t, p, b, mb, nb);
-      const int n_first = nb * BN + col_half * (BN / 2);
-      BiasRegs<BN / 2> br;
-      bias_prefetch(br, n_first, p, lane);
+      typename Epi::template Pre<BN> pre;
+      Epi::template prefetch<BN>(pre, nb, col_half, p, lane);
       int ready = 0;
       if (lane == 0)
         ready = mbar_wait(smem_u32(&bars->tmem_full[buf]), tph, wctx, kStatusTimeoutEpilogue) ? 1 : 0;
       ready = __shfl_sync(0xffffffffu, ready, 0);
       if (!ready) break;
       tc_fence_after();
-      const uint32_t taddr =
-          tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN + col_half * (BN / 2);
-      epilogue_warp<BN / 2, OutT>(taddr, n_first, mb * kBM + quarter * 32, b, p, &tma_c, stage_buf, lane, br, [&] {
-                                    tc_fence_before();
-                                    __syncwarp();
-                                    if (lane == 0) mbar_arrive(smem_u32(&bars->tmem_empty[buf]));
-                                  });
+      const uint32_t tacc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN;
+      Epi::template run<BN>(tacc, nb, col_half, mb * kBM + quarter * 32, b, p, &tma_c, stage_buf, lane, pre, [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bars->tmem_empty[buf]));
+      });
     }
     // The staged stores have read their shared-memory source before the CTA's
     // shared memory goes away; their global writes drain on their own.
@@ -710,10 +763,11 @@ constexpr int tc_pair_smem_bytes() {
          static_cast<int>(sizeof(TcBarriers<STAGES>));
 }
 
-template <int BN, int STAGES, class Loader, typename OutT>
+template <int BN, int STAGES, class Loader, class Epi>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    tc_gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
-                        const __grid_constant__ CUtensorMap tma_c, const TcParams p) {
+    tc_gemm_pair_kernel(const __grid_constant__ typename Loader::MapA tma_a,
+                        const __grid_constant__ typename Loader::MapB tma_b,
+                        const __grid_constant__ typename Epi::MapC tma_c, const typename Epi::Params p) {
   constexpr int BNL = BN / 2;  // B columns this CTA stages
   constexpr uint32_t kAStage = kBM * kBK * 2;
   constexpr uint32_t kBStage = BNL * kBK * 2;
@@ -862,29 +916,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const uint32_t tph = (local >> 1) & 1;
       int b, mb, nb;
       tile_coords(t, p, b, mb, nb);
-      const int n_first = nb * BN + col_half * (BN / 2);
-      BiasRegs<BN / 2> br;
-      bias_prefetch(br, n_first, p, lane);
+      typename Epi::template Pre<BN> pre;
+      Epi::template prefetch<BN>(pre, nb, col_half, p, lane);
       int ready = 0;
       if (lane == 0)
         ready = mbar_wait(smem_u32(&bars->tmem_full[buf]), tph, wctx, kStatusTimeoutEpilogue) ? 1 : 0;
       ready = __shfl_sync(0xffffffffu, ready, 0);
       if (!ready) break;
       tc_fence_after();
-      const uint32_t taddr =
-          tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN + col_half * (BN / 2);
-      epilogue_warp<BN / 2, OutT>(taddr, n_first, mb * (2 * kBM) + static_cast<int>(rank) * kBM + quarter * 32, b,
-                                  p, &tma_c, stage_buf, lane, br, [&] {
-                                    tc_fence_before();
-                                    __syncwarp();
-                                    if (lane == 0) {
-                                      const uint32_t eb = smem_u32(&bars->tmem_empty[buf]);
-                                      if (leader)
-                                        mbar_arrive(eb);
-                                      else
-                                        mbar_arrive_cluster(mapa_shared(eb, 0));
-                                    }
-                                  });
+      const uint32_t tacc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN;
+      Epi::template run<BN>(tacc, nb, col_half, mb * (2 * kBM) + static_cast<int>(rank) * kBM + quarter * 32, b, p,
+                            &tma_c, stage_buf, lane, pre, [&] {
+                              tc_fence_before();
+                              __syncwarp();
+                              if (lane == 0) {
+                                const uint32_t eb = smem_u32(&bars->tmem_empty[buf]);
+                                if (leader)
+                                  mbar_arrive(eb);
+                                else
+                                  mbar_arrive_cluster(mapa_shared(eb, 0));
+                              }
+                            });
     }
     // The staged stores have read their shared-memory source before the CTA's
     // shared memory goes away; their global writes drain on their own.
@@ -949,11 +1001,11 @@ constexpr int tc_wide_smem_bytes() {
          static_cast<int>(sizeof(TcWideBarriers<STAGES>));
 }
 
-template <int STAGES, class Loader, typename OutT>
+template <int STAGES, class Loader, class Epi>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    tc_gemm_pair_wide_kernel(const __grid_constant__ CUtensorMap tma_a,
-                             const __grid_constant__ CUtensorMap tma_b,
-                             const __grid_constant__ CUtensorMap tma_c, const TcParams p) {
+    tc_gemm_pair_wide_kernel(const __grid_constant__ typename Loader::MapA tma_a,
+                             const __grid_constant__ typename Loader::MapB tma_b,
+                             const __grid_constant__ typename Epi::MapC tma_c, const typename Epi::Params p) {
   constexpr int BN = 256;
   constexpr int BNL = 128;
   constexpr uint32_t kAHalf = kBM * kBK * 2;   // 128 rows x 64 (16 KB)
@@ -1187,9 +1239,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (int64_t t = cluster_id; t < p.num_tiles && ok; t += num_clusters, ++local) {
       int b, mb, nb;
       tile_coords(t, p, b, mb, nb);
-      const int n_first = nb * BN + col_half * (BN / 2);  // the same columns for both halves
-      BiasRegs<BN / 2> br;
-      bias_prefetch(br, n_first, p, lane);
+      typename Epi::template Pre<BN> pre;  // the same columns for both halves
+      Epi::template prefetch<BN>(pre, nb, col_half, p, lane);
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {
         int ready = 0;
@@ -1201,21 +1252,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           break;
         }
         tc_fence_after();
-        const uint32_t taddr =
-            tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + h * BN + col_half * (BN / 2);
-        epilogue_warp<BN / 2, OutT>(taddr, n_first,
-                                    mb * (4 * kBM) + static_cast<int>(rank) * (2 * kBM) + h * kBM + quarter * 32,
-                                    b, p, &tma_c, stage_buf, lane, br, [&] {
-                                      tc_fence_before();
-                                      __syncwarp();
-                                      if (lane == 0) {
-                                        const uint32_t eb = smem_u32(&bars->tmem_empty[h]);
-                                        if (leader)
-                                          mbar_arrive(eb);
-                                        else
-                                          mbar_arrive_cluster(mapa_shared(eb, 0));
-                                      }
-                                    });
+        const uint32_t tacc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + h * BN;
+        Epi::template run<BN>(tacc, nb, col_half,
+                              mb * (4 * kBM) + static_cast<int>(rank) * (2 * kBM) + h * kBM + quarter * 32, b, p,
+                              &tma_c, stage_buf, lane, pre, [&] {
+                                tc_fence_before();
+                                __syncwarp();
+                                if (lane == 0) {
+                                  const uint32_t eb = smem_u32(&bars->tmem_empty[h]);
+                                  if (leader)
+                                    mbar_arrive(eb);
+                                  else
+                                    mbar_arrive_cluster(mapa_shared(eb, 0));
+                                }
+                              });
       }
     }
     // The staged stores have read their shared-memory source before the CTA's

@@ -85,7 +85,8 @@ typedef struct choreo_gemm_desc {
  * reference's get_optimal_gemm_config, compute/compute_impl.hpp:74-91, and the
  * auto_analyze() of examples/ideal_matmul_example.cu:244-290). */
 typedef struct choreo_launch_config {
-  int32_t kernel;          /* 1 = tcgen05 tile GEMM, 2 = CUDA-core f32 GEMM, 3 = tcgen05 conv */
+  int32_t kernel;          /* 1 = tcgen05 tile GEMM, 2 = CUDA-core f32 GEMM, 3 = tcgen05 conv,
+                              4 = gated feed-forward product, 5 = 8-bit block-scaled GEMM */
   int32_t tile_m, tile_n, tile_k;
   int32_t stages;          /* shared-memory pipeline depth */
   int32_t cluster_m;       /* CTAs per cluster along M (1 = no cluster) */
@@ -259,6 +260,179 @@ int choreo_gemm_rowsharded(const choreo_gemm_desc* descs, int ngpu, const int* d
  * slab may end in a partial tile), tile counts differing by at most one,
  * earlier shards taking the extra tiles. */
 int choreo_shard_rows(int64_t m, int nshards, int rank, int64_t* row0, int64_t* rows);
+
+/* ---- gated feed-forward product ------------------------------------------
+ * The two input projections of a gated feed-forward block, its activation and
+ * the product, in one kernel, and their backward pass. They stand beside
+ * choreo_gemm: same operand rules, same workspace and error conventions. The
+ * reference has no counterpart (its only fused epilogue is documented, not
+ * defined; relu is a separate pass, choreo-ir.hpp:196-222). */
+
+typedef enum choreo_activation {
+  CHOREO_ACT_SILU = 0,       /* g / (1 + exp(-g)) */
+  CHOREO_ACT_GELU = 1,       /* g * Phi(g), Phi the normal distribution function */
+  CHOREO_ACT_GELU_TANH = 2,  /* g / 2 * (1 + tanh(sqrt(2/pi) * (g + 0.044715 g^3))) */
+  CHOREO_ACT_RELU = 3        /* max(g, 0); slope 0 at g = 0 */
+} choreo_activation;
+
+/* H = act(X Wg) * (X Wu), element by element, for m rows (tokens) of X:
+ *   X M x K (ldx >= K), H M x N (ldh >= N), row-major;
+ *   Wg and Wu: trans_w == 0 -> K x N row-major (ldw >= N), trans_w != 0 ->
+ *   N x K row-major (ldw >= K); they may be two parts of one matrix.
+ * gate and up (both NULL, or both given) receive X Wg and X Wu, M x N with
+ * leading dimension ld_gu >= N, for the backward pass.
+ * dtype (f16 or bf16) is the type of all of them; products are summed in fp32
+ * and the activation is computed from the unrounded sums. Outputs must not
+ * overlap one another or the inputs. */
+typedef struct choreo_ffn_desc {
+  int64_t m, n, k;
+  int32_t dtype;
+  int32_t act;                 /* choreo_activation */
+  const void* x;
+  int64_t ldx;
+  const void* w_gate;
+  const void* w_up;
+  int64_t ldw;
+  int32_t trans_w;
+  int32_t reserved;            /* 0 */
+  void* h;
+  int64_t ldh;
+  void* gate;
+  void* up;
+  int64_t ld_gu;
+} choreo_ffn_desc;
+
+/* The backward pass of choreo_gated_ffn from dH, the gradient of H. With
+ * G = X Wg and U = X Wu:
+ *   dG = dH * U * act'(G), dU = dH * act(G), each rounded to dtype;
+ *   dX = dG Wg^T + dU Wu^T (one fp32 sum), dWg = X^T dG, dWu = X^T dU, the
+ *   latter two laid out like the weights (trans_w, ld_dw).
+ * gate and up are what the forward call kept; both NULL computes them again
+ * from X (in fp32, not rounded), at half as much more work and without their
+ * 2 M N elements of memory.
+ * dx, and dw_gate with dw_up, may be NULL: that part is left out. h (NULL:
+ * left out) receives H again. dtype_dw is dtype or f32; accumulate_dw != 0
+ * adds to what dw_gate and dw_up hold. dX and H have the type dtype. Outputs
+ * must not overlap one another or the inputs. */
+typedef struct choreo_ffn_grad_desc {
+  int64_t m, n, k;
+  int32_t dtype;
+  int32_t act;
+  const void* x;
+  int64_t ldx;
+  const void* w_gate;
+  const void* w_up;
+  int64_t ldw;
+  int32_t trans_w;
+  int32_t dtype_dw;
+  const void* dh;
+  int64_t ld_dh;
+  const void* gate;
+  const void* up;
+  int64_t ld_gu;
+  void* dx;
+  int64_t ld_dx;
+  void* dw_gate;
+  void* dw_up;
+  int64_t ld_dw;
+  int32_t accumulate_dw;
+  int32_t reserved;            /* 0 */
+  void* h;
+  int64_t ldh;
+} choreo_ffn_grad_desc;
+
+/* Validates `d` and reports the kernel configuration (kernel 4; tile_n counts
+ * columns of H) and the workspace size: repacks of operands whose base or
+ * leading dimension is not 16-byte aligned. */
+int choreo_gated_ffn_query(const choreo_ffn_desc* d, choreo_launch_config* out);
+
+/* Enqueues the forward product on `stream`; `workspace` as for choreo_gemm. */
+int choreo_gated_ffn(const choreo_ffn_desc* d, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Validates `d` and reports the workspace the backward pass needs: dG and dU
+ * (2 M N elements), operand repacks, and fp32 partials when the sum over 2 N
+ * of dX is split (workspace_min_bytes: without the partials, dX then runs
+ * unsplit). The launch fields describe the product that makes dX. */
+int choreo_gated_ffn_backward_query(const choreo_ffn_grad_desc* d, choreo_launch_config* out);
+
+/* Enqueues the backward pass on `stream`. The workspace is in use until the
+ * stream has passed the call; calls that may overlap on the GPU (two streams,
+ * two captured graphs) need one each. Results are the same bit for bit on
+ * every run. */
+int choreo_gated_ffn_backward(const choreo_ffn_grad_desc* d, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- 8-bit operands with a scale for each block --------------------------- */
+
+/* Quantises op(X) (X rows x cols row-major, ldx >= cols; op the transpose when
+ * transpose != 0) to e4m3 with one fp32 scale per block of block_rows (1 or
+ * 128) rows by 128 columns of op(X). For each block, with
+ * a = max(largest finite |x|, 2^-100), every step rounded to fp32:
+ *   scale = a / 448,   q = e4m3(x * (448 / a)), ties to even,
+ * so x = q * scale within e4m3's rounding; a NaN or infinite x becomes NaN and
+ * leaves its block's scale alone. q is op(X)'s rows, one byte each, with
+ * leading dimension ldq; the scale of block (i, j) goes to
+ * scale[i * scale_row + j * scale_blk]. scale_row = 1 with
+ * scale_blk >= the number of block rows (the scales of one column block side
+ * by side) is what choreo_gemm_block_scaled reads fastest. */
+typedef struct choreo_quant_desc {
+  int64_t rows, cols;
+  int32_t dtype;               /* f16, bf16 or f32 */
+  int32_t transpose;
+  const void* x;
+  int64_t ldx;
+  int32_t block_rows;          /* 1 or 128 */
+  int32_t reserved;            /* 0 */
+  void* q;
+  int64_t ldq;
+  float* scale;
+  int64_t scale_row, scale_blk;
+} choreo_quant_desc;
+
+/* Enqueues the quantisation on `stream`. rows == 0 or cols == 0 does nothing. */
+int choreo_quantize_block(const choreo_quant_desc* d, void* stream);
+
+/* C = act(alpha * S + beta * D + bias) with
+ *   S[i,j] = sum over blocks t of scale_a(i, t) * scale_b(j, t)
+ *            * sum over k in block t of A[i,k] * B[j,k]
+ * A is M x K and B is N x K, e4m3, both K-contiguous (lda, ldb >= K and, like
+ * the base addresses, multiples of 16 bytes: choreo_quantize_block makes both,
+ * transposed where an operand is stored the other way round); blocks are 128
+ * long along K (the last one may be shorter). scale_a(i, t) =
+ * scale_a[i * scale_a_row + t * scale_a_blk]; scale_b(j, t) =
+ * scale_b[(j / block_b) * scale_b_row + t * scale_b_blk], block_b 1 or 128.
+ * D is `addend` (M x N of C's type, ld_addend >= N), or C itself when it is
+ * NULL; it is read only when beta != 0. bias and relu as in choreo_gemm_desc.
+ * Each block's product is summed by the tensor cores and added to an fp32 sum
+ * of all blocks. C is f16, bf16 or f32 and must not overlap the inputs. */
+typedef struct choreo_gemm_block_desc {
+  int64_t m, n, k;
+  const void* a;
+  int64_t lda;
+  const float* scale_a;
+  int64_t scale_a_row, scale_a_blk;
+  const void* b;
+  int64_t ldb;
+  const float* scale_b;
+  int64_t scale_b_row, scale_b_blk;
+  int32_t block_b;             /* 1 or 128 */
+  int32_t dtype_c;
+  void* c;
+  int64_t ldc;
+  float alpha;
+  float beta;
+  const void* addend;
+  int64_t ld_addend;
+  const void* bias;
+  int32_t dtype_bias;
+  int32_t relu;
+} choreo_gemm_block_desc;
+
+/* Validates `d` and reports the kernel configuration (kernel 5). The call
+ * needs no workspace. */
+int choreo_gemm_block_scaled_query(const choreo_gemm_block_desc* d, choreo_launch_config* out);
+
+/* Enqueues the product on `stream`. */
+int choreo_gemm_block_scaled(const choreo_gemm_block_desc* d, void* stream);
 
 /* ---- convolution ------------------------------------------------------- */
 
