@@ -217,13 +217,15 @@ struct GateParams : TcParams {
 
 // One warp's kCols columns of one 16-bit output, packed in pairs: through the
 // staging buffer and a bulk tensor store when the columns fill its 128-byte
-// rows and the output is TMA-addressable, else 16-byte vectors or elements.
+// rows and the output is TMA-addressable, else 16-byte vectors or elements. (A
+// bulk tensor store clips columns in whole 16 bytes, so it is not used where
+// the matrix ends inside 16 bytes.)
 template <int kCols, typename OutT>
 __device__ __forceinline__ void gate_store(const uint32_t (&q)[kCols / 32][16], const CUtensorMap* map, bool tma,
                                            bool vec, void* base, int64_t ld, int h0, int row0, int m, int n,
                                            uint32_t stage_buf, int lane) {
   if constexpr (kCols == 64) {
-    if (tma) {
+    if (tma && (h0 + 64 <= n || n % 8 == 0)) {
       if (lane == 0) bulk_wait_read_all();  // the warp's previous store has read the buffer
       __syncwarp();
       const uint32_t row_addr = stage_buf + static_cast<uint32_t>(lane) * 128u;

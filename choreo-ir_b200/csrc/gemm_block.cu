@@ -12,6 +12,7 @@
 
 #include <algorithm>
 #include <cstring>
+#include <cstdlib>
 
 #include "internal.h"
 #include "tc_kernel.cuh"
@@ -31,14 +32,27 @@ struct BlockParams : TcParams {
   int32_t d_vec;
 };
 
+template <int STAGES, int BUFS>
+struct alignas(8) BlockBarriers {
+  uint64_t full[STAGES];      // the stage's tiles have landed
+  uint64_t empty[STAGES];     // its MMAs are done: the stage is free, its block's accumulator is full
+  uint64_t tmem_empty[BUFS];  // the epilogue has read the accumulator
+  uint64_t drain;
+  uint64_t probe[2];
+  uint32_t tmem_base;
+  int32_t abort;
+};
+
 template <bool PAIR, int BN>
 struct BlockShape {
   static constexpr int kBRows = PAIR ? BN / 2 : BN;  // B rows one CTA stages
   static constexpr uint32_t kAStage = kBM * kBlockK;
   static constexpr uint32_t kBStage = kBRows * kBlockK;
-  static constexpr int kStages = 6;
+  static constexpr int kStages = (PAIR ? BN / 2 : BN) == 256 ? 4 : (PAIR && BN == 128 ? 8 : 6);
+  static constexpr int kBufs = 512 / BN;  // block accumulators in TMEM
+  using Barriers = BlockBarriers<kStages, kBufs>;
   static constexpr int kSmem = kStages * static_cast<int>(kAStage + kBStage) + kStagingBytes + 1024 +
-                               static_cast<int>(sizeof(TcBarriers<kStages>));
+                               static_cast<int>(sizeof(Barriers));
   // 128 sums a thread and two 32-column reads in flight need more registers
   // than an even share of the SM's
   static constexpr bool kMoveRegs = BN == 256;
@@ -52,12 +66,19 @@ __device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
   return r;
 }
-// (d0, d1) += (a0, a1) * (s0, s1), one rounding per element.
-__device__ __forceinline__ void fma2_acc(float& d0, float& d1, uint32_t a0, uint32_t a1, uint64_t s) {
-  uint64_t d = pack_f32x2(d0, d1);
-  const uint64_t a = pack_f32x2(__uint_as_float(a0), __uint_as_float(a1));
+// A load the compiler leaves where it is written: ahead of a wait, not next to
+// the use of its value.
+__device__ __forceinline__ float ldg_early(const float* p) {
+  float v;
+  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+
+// d += (a0, a1) * s on packed pairs, one rounding per element.
+__device__ __forceinline__ void fma2_acc(uint64_t& d, uint32_t a0, uint32_t a1, uint64_t s) {
+  uint64_t a;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "r"(a0), "r"(a1));
   asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(s));
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(d0), "=f"(d1) : "l"(d));
 }
 __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   uint64_t r;
@@ -70,7 +91,7 @@ __device__ __forceinline__ void ld_shared_2x64(uint32_t addr, uint64_t& a, uint6
 
 // Writes one warp's 32 rows x kCols columns of sums.
 template <int kCols, typename OutT>
-__device__ __forceinline__ void block_output(const float (&acc)[kCols], int n_first, int row0, const BlockParams& p,
+__device__ __forceinline__ void block_output(const uint64_t (&acc)[kCols / 2], int n_first, int row0, const BlockParams& p,
                                              const CUtensorMap* tma_c, uint32_t stage_buf, int lane) {
   constexpr int E = 128 / static_cast<int>(sizeof(OutT));  // columns per 128-byte staging row
   constexpr int kCpg = E / 32;
@@ -84,7 +105,10 @@ __device__ __forceinline__ void block_output(const float (&acc)[kCols], int n_fi
   for (int g = 0; g < kCols / E; ++g) {
     const int n_base = n_first + g * E;
     if (n_base >= p.n) break;  // warp-uniform
-    if (p.c_tma) {
+    // A bulk tensor store clips columns in whole 16 bytes: a ragged last group
+    // that ends inside 16 bytes is stored element by element.
+    const bool tma = p.c_tma != 0 && (n_base + E <= p.n || p.n * static_cast<int>(sizeof(OutT)) % 16 == 0);
+    if (tma) {
       if (lane == 0) bulk_wait_read_all();  // the warp's previous store has read the buffer
       __syncwarp();
     }
@@ -92,10 +116,11 @@ __device__ __forceinline__ void block_output(const float (&acc)[kCols], int n_fi
     for (int c = 0; c < kCpg; ++c) {
       uint32_t r[32];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(acc[g * E + c * 32 + i]);
+      for (int i = 0; i < 16; ++i)
+        asm("mov.b64 {%0, %1}, %2;" : "=r"(r[2 * i]), "=r"(r[2 * i + 1]) : "l"(acc[(g * E + c * 32) / 2 + i]));
       float v[32];
       epilogue_values<OutT>(r, v, drow, n_base + c * 32, pd, row_ok, lane);
-      if (p.c_tma) {
+      if (tma) {
         stage_row_32<OutT>(v, stage_buf + static_cast<uint32_t>(lane) * 128u, lane,
                            c * (32 * static_cast<int>(sizeof(OutT)) / 16));
       } else if (row_ok) {
@@ -104,7 +129,7 @@ __device__ __forceinline__ void block_output(const float (&acc)[kCols], int n_fi
           if (n_base + c * 32 + i < p.n) crow[n_base + c * 32 + i] = from_f32<OutT>(v[i]);
       }
     }
-    if (p.c_tma) {
+    if (tma) {
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
@@ -122,14 +147,16 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
   using S = BlockShape<PAIR, BN>;
   constexpr int STAGES = S::kStages;
   constexpr int kCols = BN / 2;  // columns of one epilogue warp
-  constexpr uint32_t kTmemCols = 2 * BN;
+  constexpr int kAhead = 1;
+  constexpr uint32_t kTmemCols = 512;
+  constexpr int kBufs = S::kBufs;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
   uint8_t* s_a = smem;
   uint8_t* s_b = smem + STAGES * S::kAStage;
   uint8_t* s_stage = s_b + STAGES * S::kBStage;
-  auto* bars = reinterpret_cast<TcBarriers<STAGES>*>(s_stage + kStagingBytes);
+  auto* bars = reinterpret_cast<typename S::Barriers*>(s_stage + kStagingBytes);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0;
@@ -143,8 +170,7 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
       mbar_init(smem_u32(&bars->full[s]), 1);
       mbar_init(smem_u32(&bars->empty[s]), 1);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_u32(&bars->tmem_full[i]), 1);
+    for (int i = 0; i < kBufs; ++i) {
       mbar_init(smem_u32(&bars->tmem_empty[i]), (PAIR ? 2 : 1) * kEpiWarps);
     }
     mbar_init(smem_u32(&bars->drain), 1);
@@ -214,47 +240,48 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
           }
         }
       }
-    } else if (warp == 1 && leader && lane == 0) {
+    } else if (warp == 1 && leader) {
       // ---------------------------------------------------------- MMA issuer
-      const uint32_t idesc = idesc_e4m3(kTileM, BN);
-      uint32_t stage = 0, phase = 0, blocks = 0;
-      bool ok = true;
-      for (int64_t t = first; t < p.num_tiles && ok; t += step) {
-        for (int kb = 0; kb < p.num_k_blocks; ++kb, ++blocks) {
-          const uint32_t buf = blocks & 1;
-          if (!mbar_wait(smem_u32(&bars->tmem_empty[buf]), ((blocks >> 1) & 1) ^ 1, wctx, kStatusTimeoutMma) ||
-              !mbar_wait(smem_u32(&bars->full[stage]), phase, wctx, kStatusTimeoutMma)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t a0 = smem_u32(s_a + stage * S::kAStage);
-          const uint32_t b0 = smem_u32(s_b + stage * S::kBStage);
+      // The whole warp runs the loop and one lane issues: operands that are the
+      // same in every lane stay in uniform registers, where the MMA wants them.
+      // Its chain of dependent instructions is what a short k-block waits for,
+      // so it holds little: descriptors and barrier addresses
+      // advance by additions, and one commit per k-block tells the producer
+      // that the stage is free and the epilogue that its accumulator is full.
+      constexpr uint32_t idesc = idesc_e4m3(kTileM, BN);
+      const uint64_t desc_a = smem_desc_sw128(smem_u32(s_a), 16, 1024);
+      const uint64_t desc_b = smem_desc_sw128(smem_u32(s_b), 16, 1024);
+      const uint32_t bar_full = smem_u32(&bars->full[0]), bar_done = smem_u32(&bars->empty[0]);
+      const uint32_t bar_free = smem_u32(&bars->tmem_empty[0]);
+      uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 1;
+      const int64_t blocks = (p.num_tiles - first + step - 1) / step * p.num_k_blocks;
+      for (int64_t i = 0; i < blocks; ++i) {
+        const bool ready = mbar_wait(bar_full + 8 * stage, phase, wctx, kStatusTimeoutMma) &&
+                           mbar_wait(bar_free + 8 * buf, buf_phase, wctx, kStatusTimeoutMma);
+        if (!__all_sync(0xffffffffu, ready)) break;
+        tc_fence_after();
+        const uint64_t ad = smem_desc_advance(desc_a, stage * S::kAStage);
+        const uint64_t bd = smem_desc_advance(desc_b, stage * S::kBStage);
+        const uint32_t d = tmem_base + buf * BN;
+        if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < kBlockK / 32; ++k) {
-            const uint64_t ad = smem_desc_sw128(a0 + k * 32, 16, 1024);
-            const uint64_t bd = smem_desc_sw128(b0 + k * 32, 16, 1024);
+          for (uint32_t k = 0; k < kBlockK / 32; ++k) {
             if constexpr (PAIR)
-              umma_f8_pair(tmem_base + buf * BN, ad, bd, idesc, k != 0 ? 1u : 0u);
+              umma_f8_pair(d, smem_desc_advance(ad, k * 32), smem_desc_advance(bd, k * 32), idesc, k != 0 ? 1u : 0u);
             else
-              umma_f8(tmem_base + buf * BN, ad, bd, idesc, k != 0 ? 1u : 0u);
+              umma_f8(d, smem_desc_advance(ad, k * 32), smem_desc_advance(bd, k * 32), idesc, k != 0 ? 1u : 0u);
           }
-          const uint32_t eb = smem_u32(&bars->empty[stage]);
-          const uint32_t tf = smem_u32(&bars->tmem_full[buf]);
-          if constexpr (PAIR) {
-            umma_commit_pair(eb);
-            umma_commit_pair(mapa_shared(eb, 1));
-            umma_commit_pair(tf);
-            umma_commit_pair(mapa_shared(tf, 1));
-          } else {
-            umma_commit(eb);
-            umma_commit(tf);
-          }
-          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+          if constexpr (PAIR) umma_commit_pair_both(bar_done + 8 * stage); else umma_commit(bar_done + 8 * stage);
         }
+        __syncwarp();
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        if (++buf == kBufs) { buf = 0; buf_phase ^= 1; }
       }
-      if constexpr (PAIR) umma_commit_pair(smem_u32(&bars->drain)); else umma_commit(smem_u32(&bars->drain));
+      if (elect_one()) {
+        if constexpr (PAIR) umma_commit_pair(smem_u32(&bars->drain)); else umma_commit(smem_u32(&bars->drain));
+      }
       mbar_wait(smem_u32(&bars->drain), 0, wctx, kStatusTimeoutDrain, false);
+      __syncwarp();
     }
   } else {
     if constexpr (S::kMoveRegs) regs_inc<S::kEpiRegs>();
@@ -262,8 +289,11 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
     const int quarter = warp & 3;
     const int col_half = (warp - 4) >> 2;
     const uint32_t stage_buf = smem_u32(s_stage) + static_cast<uint32_t>(warp - 4) * 4096u;
+    const uint32_t tmem_warp = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + col_half * kCols;
+    const uint32_t bar_done = smem_u32(&bars->empty[0]);
+    const uint32_t bar_free = PAIR ? mapa_shared(smem_u32(&bars->tmem_empty[0]), 0) : smem_u32(&bars->tmem_empty[0]);
     griddep_wait();
-    uint32_t blocks = 0;
+    uint32_t stage = 0, phase = 0, buf = 0;
     bool ok = true;
     for (int64_t t = first; t < p.num_tiles && ok; t += step) {
       int b, mb, nb;
@@ -282,86 +312,97 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
       } else {
         sb[0] = p.sb + static_cast<int64_t>(min(n_first, p.n - 1) / 128) * p.sb_row;
       }
-      float acc[kCols];
+      uint64_t acc[kCols / 2];  // the warp's sums, in pairs of columns
 #pragma unroll
-      for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
-      float next_a = __ldg(sa);
-      float next_b[BVEC ? kCols / 32 : 1];
+      for (int i = 0; i < kCols / 2; ++i) acc[i] = 0;
+      // Scales are loaded kAhead k-blocks before their use: one k-block takes
+      // less time than a load from L2 or HBM.
+      constexpr int kSb = BVEC ? kCols / 32 : 1;
+      float ahead_a[kAhead], ahead_b[kAhead][kSb];
+      auto load_scales = [&](int kb, float& a, float (&bv)[kSb]) {
+        if (kb >= p.num_k_blocks) return;
+        a = ldg_early(sa);
+        sa += p.sa_blk;
 #pragma unroll
-      for (int c = 0; c < (BVEC ? kCols / 32 : 1); ++c) next_b[c] = __ldg(sb[c]);
+        for (int c = 0; c < kSb; ++c) {
+          bv[c] = ldg_early(sb[c]);
+          sb[c] += p.sb_blk;
+        }
+      };
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) load_scales(i, ahead_a[i], ahead_b[i]);
       if constexpr (BVEC) {
         if (lane == 0) bulk_wait_read_all();  // the previous tile's stores have read the buffer
         __syncwarp();
       }
+      // Unrolled by kAhead so that each slot of the scale queue is a register
+      // of its own (moving a value that is still in flight would wait for it).
 #pragma unroll 1
-      for (int kb = 0; kb < p.num_k_blocks; ++kb, ++blocks) {
-        const uint32_t buf = blocks & 1;
-        const float cur_a = next_a;
+      for (int kb0 = 0; kb0 < p.num_k_blocks && ok; kb0 += kAhead) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int kb = kb0 + u;
+        if (kb >= p.num_k_blocks) break;
+        const float cur_a = ahead_a[u];
         float s = 0.f;
         uint32_t sbuf = 0;
         if constexpr (BVEC) {
           // the block's column scales, read back below as broadcasts
           sbuf = stage_buf + (kb & 1) * 512u;
 #pragma unroll
-          for (int c = 0; c < kCols / 32; ++c) st_shared_f32(sbuf + static_cast<uint32_t>(c * 32 + lane) * 4u, next_b[c]);
+          for (int c = 0; c < kSb; ++c) st_shared_f32(sbuf + static_cast<uint32_t>(c * 32 + lane) * 4u, ahead_b[u][c]);
           __syncwarp();
         } else {
-          s = cur_a * next_b[0];
+          s = cur_a * ahead_b[u][0];
         }
-        if (kb + 1 < p.num_k_blocks) {
-          next_a = __ldg(sa + static_cast<int64_t>(kb + 1) * p.sa_blk);
-#pragma unroll
-          for (int c = 0; c < (BVEC ? kCols / 32 : 1); ++c)
-            next_b[c] = __ldg(sb[c] + static_cast<int64_t>(kb + 1) * p.sb_blk);
-        }
-        const bool ready = mbar_wait(smem_u32(&bars->tmem_full[buf]), (blocks >> 1) & 1, wctx, kStatusTimeoutEpilogue);
+        load_scales(kb + kAhead, ahead_a[u], ahead_b[u]);
+        const bool ready = mbar_wait(bar_done + 8 * stage, phase, wctx, kStatusTimeoutEpilogue);
         if (!__all_sync(0xffffffffu, ready)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t taddr =
-            tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN + col_half * kCols;
+        const uint32_t taddr = tmem_warp + buf * BN;
+        const uint32_t free_bar = bar_free + 8 * buf;
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        if (++buf == kBufs) buf = 0;
         auto release = [&] {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) {
-            const uint32_t eb = smem_u32(&bars->tmem_empty[buf]);
-            if (leader)
-              mbar_arrive(eb);
-            else
-              mbar_arrive_cluster(mapa_shared(eb, 0));
+            if constexpr (PAIR) mbar_arrive_cluster(free_bar); else mbar_arrive(free_bar);
           }
         };
         if (!active) {
           release();
           continue;
         }
-        uint32_t r[2][32];
-        tmem_ld_32x32b_x32(taddr, r[0]);
-        tmem_wait_ld(r[0]);
+        // One 32-column read at a time: the SM sub-partition's other epilogue
+        // warp works meanwhile, and a second one in flight would not fit the
+        // registers beside the sums.
 #pragma unroll
         for (int c = 0; c < kCols / 32; ++c) {
-          if (c + 1 < kCols / 32) tmem_ld_32x32b_x32(taddr + (c + 1) * 32, r[(c + 1) & 1]);
-          else release();
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(taddr + c * 32, r);
+          tmem_wait_ld(r);
+          if (c + 1 == kCols / 32) release();
           if constexpr (BVEC) {
             const uint64_t a2 = pack_f32x2(cur_a, cur_a);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               uint64_t b0, b1;
               ld_shared_2x64(sbuf + static_cast<uint32_t>(c * 32 + 4 * j) * 4u, b0, b1);
-              fma2_acc(acc[c * 32 + 4 * j], acc[c * 32 + 4 * j + 1], r[c & 1][4 * j], r[c & 1][4 * j + 1], mul2(a2, b0));
-              fma2_acc(acc[c * 32 + 4 * j + 2], acc[c * 32 + 4 * j + 3], r[c & 1][4 * j + 2], r[c & 1][4 * j + 3],
-                       mul2(a2, b1));
+              fma2_acc(acc[c * 16 + 2 * j], r[4 * j], r[4 * j + 1], mul2(a2, b0));
+              fma2_acc(acc[c * 16 + 2 * j + 1], r[4 * j + 2], r[4 * j + 3], mul2(a2, b1));
             }
           } else {
             const uint64_t s2 = pack_f32x2(s, s);
 #pragma unroll
             for (int j = 0; j < 16; ++j)
-              fma2_acc(acc[c * 32 + 2 * j], acc[c * 32 + 2 * j + 1], r[c & 1][2 * j], r[c & 1][2 * j + 1], s2);
+              fma2_acc(acc[c * 16 + j], r[2 * j], r[2 * j + 1], s2);
           }
-          if (c + 1 < kCols / 32) tmem_wait_ld(r[(c + 1) & 1]);
         }
+      }
       }
       if (ok && active) block_output<kCols, OutT>(acc, n_first, row0, p, tma_c, stage_buf, lane);
     }
@@ -405,8 +446,9 @@ struct BlockConfig {
 
 BlockConfig select_block_config(int64_t m, int64_t n) {
   const int sms = current_sm_count();
-  const int64_t pairs = ((m + 255) / 256) * ((n + 255) / 256);
-  return pairs * 2 >= sms ? BlockConfig{true, 256} : BlockConfig{false, 128};
+  const int64_t wide = ((m + 127) / 128) * ((n + 255) / 256);
+  if (const char* e = getenv("TB")) return BlockConfig{e[0] == 'p', atoi(e + 1)};
+  return wide >= sms ? BlockConfig{false, 256} : BlockConfig{false, 128};
 }
 
 template <typename Kern>
@@ -432,10 +474,20 @@ int launch_block(Kern kern, int smem, bool move_regs, std::atomic<uint64_t>& att
 template <bool BVEC, typename OutT>
 int dispatch_block(const BlockConfig& c, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc,
                    const BlockParams& kp, int grid, cudaStream_t s) {
+  if (c.pair && c.bn == 128) {
+    using S = BlockShape<true, 128>;
+    static std::atomic<uint64_t> done{0};
+    return launch_block(block_pair_kernel<128, BVEC, OutT>, S::kSmem, S::kMoveRegs, done, ta, tb, tc, kp, grid, s);
+  }
   if (c.pair) {
     using S = BlockShape<true, 256>;
     static std::atomic<uint64_t> done{0};
     return launch_block(block_pair_kernel<256, BVEC, OutT>, S::kSmem, S::kMoveRegs, done, ta, tb, tc, kp, grid, s);
+  }
+  if (c.bn == 256) {
+    using S = BlockShape<false, 256>;
+    static std::atomic<uint64_t> done{0};
+    return launch_block(block_single_kernel<256, BVEC, OutT>, S::kSmem, S::kMoveRegs, done, ta, tb, tc, kp, grid, s);
   }
   using S = BlockShape<false, 128>;
   static std::atomic<uint64_t> done{0};
@@ -527,7 +579,7 @@ int choreo_gemm_block_scaled_query(const choreo_gemm_block_desc* d, choreo_launc
   out->grid_y = out->grid_z = 1;
   out->block_x = kBlockThreads;
   out->smem_bytes = c.pair ? BlockShape<true, 256>::kSmem : BlockShape<false, 128>::kSmem;
-  out->tmem_cols = 2 * c.bn;
+  out->tmem_cols = 512;
   out->split_k = 1;
   return ok();
 }
@@ -538,7 +590,7 @@ int choreo_gemm_block_scaled(const choreo_gemm_block_desc* d, void* stream) {
   const BlockConfig c = select_block_config(d->m, d->n);
   CUtensorMap ta, tb, tc;
   if ((rc = encode_e4m3(&ta, d->a, d->m, d->k, d->lda, 128))) return rc;
-  if ((rc = encode_e4m3(&tb, d->b, d->n, d->k, d->ldb, 128))) return rc;
+  if ((rc = encode_e4m3(&tb, d->b, d->n, d->k, d->ldb, static_cast<uint32_t>(c.pair ? c.bn / 2 : c.bn)))) return rc;
   BlockParams kp;
   std::memset(&kp, 0, sizeof(kp));
   kp.m = static_cast<int32_t>(d->m);

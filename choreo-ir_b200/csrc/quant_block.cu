@@ -9,6 +9,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "internal.h"
 #include "sm100.cuh"
@@ -18,13 +19,14 @@ namespace choreo_sm100 {
 
 struct QuantParams {
   int64_t rows, cols;          // of op(X)
+  int64_t row_tiles, col_tiles;
   const void* x;
   int64_t ldx;
   uint8_t* q;
   int64_t ldq;
   float* scale;
   int64_t scale_row, scale_blk;
-  int32_t x_vec, q_vec;        // 16-byte loads of X's rows / 4-byte stores of q's rows are legal
+  int32_t q_vec;               // 8-byte stores to q's rows are legal
 };
 
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
@@ -32,38 +34,329 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  return e4m3x2(a, b) | e4m3x2(c, d) << 16;
+}
 
-// x * inv, with an infinite x made NaN (the conversion would store 448).
-__device__ __forceinline__ float scaled(float x, float inv) {
-  return fabsf(x) <= 3.4028234663852886e38f ? x * inv : __int_as_float(0x7fffffff);
-}
-__device__ __forceinline__ float finite_abs(float x) {
-  const float a = fabsf(x);
-  return a <= 3.4028234663852886e38f ? a : 0.f;
-}
+constexpr float kMaxFinite = 3.4028234663852886e38f;
 constexpr float kTinyMax = 7.888609052210118e-31f;  // 2^-100: keeps 448 / a finite
 
-__device__ __forceinline__ void factors(float amax, float& inv, float& scale) {
-  const float a = fmaxf(amax, kTinyMax);
-  inv = __fdiv_rn(448.f, a);
-  scale = __fdiv_rn(a, 448.f);
+// An infinite x becomes NaN (the conversion would store 448).
+__device__ __forceinline__ float finite_or_nan(float x) { return fabsf(x) <= kMaxFinite ? x : __int_as_float(0x7fffffff); }
+__device__ __forceinline__ float finite_abs(float x) {
+  const float a = fabsf(x);
+  return a <= kMaxFinite ? a : 0.f;
+}
+__device__ __forceinline__ float factor_of(float amax) { return __fdiv_rn(448.f, fmaxf(amax, kTinyMax)); }
+__device__ __forceinline__ float scale_of(float amax) { return __fdiv_rn(fmaxf(amax, kTinyMax), 448.f); }
+
+// One 16-byte piece of a row of X: 8 elements (4 of f32).
+template <typename T>
+struct Piece {
+  static constexpr int kElems = 16 / static_cast<int>(sizeof(T));
+  uint32_t w[4];
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[i]);
+    } else {
+      float lo, hi;
+      unpack2(w[i / 2], lo, hi, static_cast<T*>(nullptr));
+      return (i & 1) ? hi : lo;
+    }
+  }
+  // Elements past `left` read as zero.
+  __device__ __forceinline__ void load(const T* p, int64_t left) {
+    if (left >= kElems) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+      return;
+    }
+    w[0] = w[1] = w[2] = w[3] = 0;
+#pragma unroll
+    for (int i = 0; i < kElems; ++i)
+      if (i < left) {
+        if constexpr (sizeof(T) == 4)
+          w[i] = __float_as_uint(p[i]);
+        else
+          w[i / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + i)) << (16 * (i & 1));
+      }
+  }
+  // Largest magnitude, as ordered bits: two 16-bit halves or one 32-bit value.
+  __device__ __forceinline__ uint32_t top() const {
+    if constexpr (sizeof(T) == 4) {
+      return max(max(w[0] & 0x7fffffffu, w[1] & 0x7fffffffu), max(w[2] & 0x7fffffffu, w[3] & 0x7fffffffu));
+    } else {
+      return __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+    }
+  }
+  __device__ __forceinline__ float finite_top() const {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < kElems; ++i) m = fmaxf(m, finite_abs(get(i)));
+    return m;
+  }
+};
+template <typename T>
+__device__ __forceinline__ uint32_t top_max(uint32_t a, uint32_t b) {
+  if constexpr (sizeof(T) == 4)
+    return max(a, b);
+  else
+    return __vmaxu2(a, b);
+}
+// The magnitude that `top` bits stand for; *all_finite: no NaN or infinity among them.
+template <typename T>
+__device__ __forceinline__ float top_value(uint32_t top, bool* all_finite) {
+  if constexpr (sizeof(T) == 4) {
+    *all_finite = top < 0x7f800000u;
+    return __uint_as_float(top);
+  } else {
+    const uint32_t m = max(top & 0xffffu, top >> 16);
+    *all_finite = m < (std::is_same_v<T, __half> ? 0x7c00u : 0x7f80u);
+    float lo, hi;
+    unpack2(m, lo, hi, static_cast<T*>(nullptr));
+    return lo;
+  }
+}
+// kElems quantised values of a piece; `clean`: no NaN or infinity in it.
+template <typename T>
+__device__ __forceinline__ void quantize_piece(const Piece<T>& v, float inv, bool clean, uint32_t (&q)[2]) {
+  float f[Piece<T>::kElems];
+#pragma unroll
+  for (int i = 0; i < Piece<T>::kElems; ++i) f[i] = (clean ? v.get(i) : finite_or_nan(v.get(i))) * inv;
+  q[0] = e4m3x4(f[0], f[1], f[2], f[3]);
+  if constexpr (sizeof(T) == 2) q[1] = e4m3x4(f[4], f[5], f[6], f[7]);
+}
+// Stores kElems bytes of a row of q, those before column `cols`.
+template <int kElems>
+__device__ __forceinline__ void store_q(uint8_t* q, const uint32_t (&v)[2], int64_t left, bool vec) {
+  if (vec && left >= kElems) {
+    if constexpr (kElems == 8)
+      *reinterpret_cast<uint2*>(q) = make_uint2(v[0], v[1]);
+    else
+      *reinterpret_cast<uint32_t*>(q) = v[0];
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < kElems; ++i)
+    if (i < left) q[i] = static_cast<uint8_t>(v[i / 4] >> (8 * (i & 3)));
 }
 
-template <typename T>
-__device__ __forceinline__ float load_elem(const T* p) { return to_f32<T>(*p); }
-
-// Block of 128 x 128 elements of op(X) per CTA (256 threads), staged in shared
-// memory as fp32; ROWS: one scale per row (1 x 128 blocks), else one per CTA.
-// TRANS reads X's rows along op(X)'s columns.
-template <typename T, bool ROWS, bool TRANS>
-__global__ void __launch_bounds__(256) quant_tile_kernel(const QuantParams p) {
-  extern __shared__ float tile[];  // 128 rows of op(X), pitch 129
-  __shared__ float warp_max[8];
+// 1 x 128 blocks along X's rows. A block is 16 lanes' 16-byte loads (32 lanes'
+// for f32); a warp takes UNROLL consecutive 512-byte runs of one row, all loads
+// in flight at once, and 8 neighbouring rows share a CTA so that their scales
+// fall into one 32-byte sector. Bound by memory: 3 (5) bytes per element.
+template <typename T, int UNROLL>
+__global__ void __launch_bounds__(256) quant_rows_kernel(const QuantParams p, int64_t runs) {
+  constexpr int E = Piece<T>::kElems;
+  constexpr int kLanes = 128 / E;  // lanes of one block
   griddep_wait();
   griddep_launch_dependents();
-  const int64_t r0 = static_cast<int64_t>(blockIdx.y) * 128;
-  const int64_t c0 = static_cast<int64_t>(blockIdx.x) * 128;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t group = blockIdx.x / runs;
+  const int64_t r = group * 8 + warp;
+  if (r >= p.rows) return;
+  const int64_t c0 = (blockIdx.x - group * runs) * (UNROLL * 32 * E) + lane * E;
+  const T* x = static_cast<const T*>(p.x) + r * p.ldx + c0;
+  Piece<T> v[UNROLL];
+#pragma unroll
+  for (int u = 0; u < UNROLL; ++u) v[u].load(x + u * 32 * E, p.cols - c0 - u * 32 * E);
+#pragma unroll
+  for (int u = 0; u < UNROLL; ++u) {
+    const int64_t c = c0 + u * 32 * E;
+    uint32_t top = v[u].top();
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) top = top_max<T>(top, __shfl_xor_sync(0xffffffffu, top, o));
+    bool clean;
+    float amax = top_value<T>(top, &clean);
+    if (__any_sync(0xffffffffu, !clean)) {
+      float m = v[u].finite_top();
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      amax = m;
+    }
+    uint32_t q[2];
+    quantize_piece<T>(v[u], factor_of(amax), clean, q);
+    store_q<E>(p.q + r * p.ldq + c, q, p.cols - c, p.q_vec != 0);
+    if (lane % kLanes == 0 && c < p.cols) p.scale[r * p.scale_row + c / 128 * p.scale_blk] = scale_of(amax);
+  }
+}
+
+// Largest finite magnitude over the CTA's 256 threads.
+template <typename T>
+__device__ __forceinline__ float cta_amax(uint32_t top, float finite_top, uint32_t* warp_top, float* warp_finite,
+                                          bool* all_clean) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    top = top_max<T>(top, __shfl_xor_sync(0xffffffffu, top, o));
+    finite_top = fmaxf(finite_top, __shfl_xor_sync(0xffffffffu, finite_top, o));
+  }
+  if (lane == 0) {
+    warp_top[warp] = top;
+    warp_finite[warp] = finite_top;
+  }
+  __syncthreads();
+  float m = 0.f;
+  bool all = true;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    bool clean;
+    top_value<T>(warp_top[w], &clean);
+    all = all && clean;
+    m = fmaxf(m, warp_finite[w]);
+  }
+  *all_clean = all;
+  return m;
+}
+
+// One 128 x 128 tile of op(X) per CTA. SQUARE: one scale for the tile, else one
+// per row of op(X).
+//
+// TRANS: the tile is loaded along X's rows (op(X)'s columns) and turned in
+// shared memory. There each row of op(X) is cut into 16-byte chunks (8 rows of
+// X, 4 for f32), chunk j of row c stored at j ^ (c / elements per load): a
+// warp's store touches 4 words of a chunk in 8 different chunks, its load of
+// whole chunks 8 different chunks per 8 lanes, both without bank conflicts.
+template <typename T, bool SQUARE, bool TRANS>
+__global__ void __launch_bounds__(256) quant_tile_kernel(const QuantParams p) {
+  constexpr int E = Piece<T>::kElems;        // elements of a load; rows of X in a chunk
+  constexpr int kPieces = 128 * 128 / E / 256;
+  constexpr int kLanes = 128 / E;
+  constexpr int kWords = 128 * static_cast<int>(sizeof(T)) / 4;  // 32-bit words of a tile row
+  extern __shared__ uint4 turned_raw[];
+  uint32_t* turned = reinterpret_cast<uint32_t*>(turned_raw);
+  __shared__ uint32_t warp_top[8];
+  __shared__ float warp_finite[8];
+  griddep_wait();
+  griddep_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t rt = blockIdx.x / p.col_tiles, ct = blockIdx.x - rt * p.col_tiles;
+  const int64_t r0 = rt * 128, c0 = ct * 128;
+  const T* x = static_cast<const T*>(p.x);
+  Piece<T> v[kPieces];
+  if constexpr (!TRANS) {
+    // piece i of the thread: row i * 8 * rows-per-warp + ..., kLanes lanes a row
+    constexpr int kRows = 32 / kLanes;  // rows of one warp load
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int64_t r = r0 + (i * 8 + warp) * kRows + lane / kLanes;
+      const int64_t c = c0 + lane % kLanes * E;
+      v[i].load(x + (r < p.rows ? r : p.rows - 1) * p.ldx + c, r < p.rows ? p.cols - c : 0);
+    }
+  } else {
+    // A warp load covers 8 pieces of 4 rows of X: 4 words (row pairs for 16
+    // bits) of one chunk. 16-bit loads come in pairs of rows.
+    constexpr int kGroups = kLanes / 8;      // 8-piece groups across the tile
+    constexpr int kPair = 4 / static_cast<int>(sizeof(T)) ;  // rows of X in one word
+#pragma unroll
+    for (int i = 0; i < kPieces / kPair; ++i) {
+      const int unit = i * 8 + warp;         // (chunk, group)
+      const int chunk = unit / kGroups, grp = unit % kGroups;
+#pragma unroll
+      for (int h = 0; h < kPair; ++h) {
+        const int64_t k = c0 + chunk * E + (lane >> 3) * kPair + h;  // row of X
+        const int64_t r = r0 + (grp * 8 + (lane & 7)) * E;           // column of X
+        v[i * kPair + h].load(x + (k < p.cols ? k : p.cols - 1) * p.ldx + r, k < p.cols ? p.rows - r : 0);
+      }
+    }
+  }
+  float inv = 0.f;
+  bool clean = true;
+  if constexpr (SQUARE) {
+    uint32_t top = 0;
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      top = top_max<T>(top, v[i].top());
+    }
+    bool own_clean;
+    m = top_value<T>(top, &own_clean);
+    if (!own_clean) {
+      m = 0.f;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) m = fmaxf(m, v[i].finite_top());
+    }
+    const float amax = cta_amax<T>(top, m, warp_top, warp_finite, &clean);
+    inv = factor_of(amax);
+    if (threadIdx.x == 0) p.scale[rt * p.scale_row + ct * p.scale_blk] = scale_of(amax);
+  }
+  if constexpr (!TRANS) {
+    static_assert(TRANS || SQUARE, "rows of X as they lie are quant_rows_kernel's");
+    constexpr int kRows = 32 / kLanes;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int64_t r = r0 + (i * 8 + warp) * kRows + lane / kLanes;
+      const int64_t c = c0 + lane % kLanes * E;
+      if (r >= p.rows) continue;
+      uint32_t q[2];
+      quantize_piece<T>(v[i], inv, clean, q);
+      store_q<E>(p.q + r * p.ldq + c, q, p.cols - c, p.q_vec != 0);
+    }
+  } else {
+    constexpr int kGroups = kLanes / 8;
+    constexpr int kPair = 4 / static_cast<int>(sizeof(T));
+#pragma unroll
+    for (int i = 0; i < kPieces / kPair; ++i) {
+      const int unit = i * 8 + warp;
+      const int chunk = unit / kGroups, grp = unit % kGroups;
+      const int piece = grp * 8 + (lane & 7);  // columns of X piece * E .. + E - 1
+      uint32_t* dst = turned + piece * E * kWords + ((chunk ^ piece) * 4 + (lane >> 3));
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        uint32_t w;
+        if constexpr (sizeof(T) == 4)
+          w = v[i].w[e];
+        else
+          w = __byte_perm(v[2 * i].w[e / 2], v[2 * i + 1].w[e / 2], (e & 1) ? 0x7632 : 0x5410);
+        dst[e * kWords] = w;
+      }
+    }
+    __syncthreads();
+    constexpr int kRows = 32 / kLanes;  // rows of op(X) of one warp load
+    const int part = lane % kLanes;
+#pragma unroll 4
+    for (int i = 0; i < 128 / 8 / kRows; ++i) {
+      const int row = (i * 8 + warp) * kRows + lane / kLanes;
+      Piece<T> u;
+      const uint4 w = *reinterpret_cast<const uint4*>(turned + row * kWords + (part ^ (row / E)) * 4);
+      u.w[0] = w.x, u.w[1] = w.y, u.w[2] = w.z, u.w[3] = w.w;
+      if constexpr (!SQUARE) {
+        uint32_t top = u.top();
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) top = top_max<T>(top, __shfl_xor_sync(0xffffffffu, top, o));
+        float amax = top_value<T>(top, &clean);
+        if (__any_sync(0xffffffffu, !clean)) {
+          float m = u.finite_top();
+#pragma unroll
+          for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+          amax = m;
+        }
+        inv = factor_of(amax);
+        if (part == 0 && r0 + row < p.rows) p.scale[(r0 + row) * p.scale_row + ct * p.scale_blk] = scale_of(amax);
+      }
+      const int64_t c = c0 + part * E;
+      if (r0 + row < p.rows) {
+        uint32_t q[2];
+        quantize_piece<T>(u, inv, clean, q);
+        store_q<E>(p.q + (r0 + row) * p.ldq + c, q, p.cols - c, p.q_vec != 0);
+      }
+    }
+  }
+}
+
+// Any alignment of X: the same tile through shared memory as f32, element by
+// element.
+template <typename T, bool SQUARE, bool TRANS>
+__global__ void __launch_bounds__(256) quant_unaligned_kernel(const QuantParams p) {
+  extern __shared__ uint4 turned_raw[];
+  float* tile = reinterpret_cast<float*>(turned_raw);  // 128 rows of op(X), pitch 129
+  __shared__ uint32_t warp_top[8];
+  __shared__ float warp_finite[8];
+  griddep_wait();
+  griddep_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t rt = blockIdx.x / p.col_tiles, ct = blockIdx.x - rt * p.col_tiles;
+  const int64_t r0 = rt * 128, c0 = ct * 128;
   const T* x = static_cast<const T*>(p.x);
   for (int i = warp; i < 128; i += 8) {
 #pragma unroll
@@ -71,30 +364,24 @@ __global__ void __launch_bounds__(256) quant_tile_kernel(const QuantParams p) {
       const int c = lane + 32 * j;
       if constexpr (!TRANS) {
         const bool in = r0 + i < p.rows && c0 + c < p.cols;
-        tile[i * 129 + c] = in ? load_elem(x + (r0 + i) * p.ldx + c0 + c) : 0.f;
+        tile[i * 129 + c] = in ? to_f32<T>(x[(r0 + i) * p.ldx + c0 + c]) : 0.f;
       } else {
         const bool in = c0 + i < p.cols && r0 + c < p.rows;
-        tile[c * 129 + i] = in ? load_elem(x + (c0 + i) * p.ldx + r0 + c) : 0.f;
+        tile[c * 129 + i] = in ? to_f32<T>(x[(c0 + i) * p.ldx + r0 + c]) : 0.f;
       }
     }
   }
   __syncthreads();
-  float inv = 0.f, scale = 0.f;
-  if constexpr (!ROWS) {
+  float inv = 0.f;
+  if constexpr (SQUARE) {
     float m = 0.f;
     for (int i = warp; i < 128; i += 8)
 #pragma unroll
       for (int j = 0; j < 4; ++j) m = fmaxf(m, finite_abs(tile[i * 129 + lane + 32 * j]));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) warp_max[warp] = m;
-    __syncthreads();
-    m = warp_max[0];
-#pragma unroll
-    for (int w = 1; w < 8; ++w) m = fmaxf(m, warp_max[w]);
-    factors(m, inv, scale);
-    if (threadIdx.x == 0)
-      p.scale[static_cast<int64_t>(blockIdx.y) * p.scale_row + static_cast<int64_t>(blockIdx.x) * p.scale_blk] = scale;
+    bool clean;
+    const float amax = cta_amax<float>(0, m, warp_top, warp_finite, &clean);
+    inv = factor_of(amax);
+    if (threadIdx.x == 0) p.scale[rt * p.scale_row + ct * p.scale_blk] = scale_of(amax);
   }
   for (int i = warp; i < 128; i += 8) {
     const int64_t r = r0 + i;
@@ -102,24 +389,17 @@ __global__ void __launch_bounds__(256) quant_tile_kernel(const QuantParams p) {
     float v[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = tile[i * 129 + 4 * lane + j];
-    if constexpr (ROWS) {
+    if constexpr (!SQUARE) {
       float m = fmaxf(fmaxf(finite_abs(v[0]), finite_abs(v[1])), fmaxf(finite_abs(v[2]), finite_abs(v[3])));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      factors(m, inv, scale);
-      if (lane == 0) p.scale[r * p.scale_row + static_cast<int64_t>(blockIdx.x) * p.scale_blk] = scale;
+      inv = factor_of(m);
+      if (lane == 0) p.scale[r * p.scale_row + ct * p.scale_blk] = scale_of(m);
     }
-    const uint32_t w = e4m3x2(scaled(v[0], inv), scaled(v[1], inv)) |
-                       e4m3x2(scaled(v[2], inv), scaled(v[3], inv)) << 16;
+    const uint32_t w[2] = {e4m3x4(finite_or_nan(v[0]) * inv, finite_or_nan(v[1]) * inv, finite_or_nan(v[2]) * inv,
+                                  finite_or_nan(v[3]) * inv), 0};
     const int64_t c = c0 + 4 * lane;
-    uint8_t* q = p.q + r * p.ldq + c;
-    if (p.q_vec && c + 4 <= p.cols) {
-      *reinterpret_cast<uint32_t*>(q) = w;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (c + j < p.cols) q[j] = static_cast<uint8_t>(w >> (8 * j));
-    }
+    store_q<4>(p.q + r * p.ldq + c, w, p.cols - c, p.q_vec != 0);
   }
 }
 
@@ -130,21 +410,46 @@ using namespace choreo_sm100;
 
 namespace {
 
-template <typename T, bool ROWS, bool TRANS>
-int launch_quant(const QuantParams& p, cudaStream_t s) {
-  constexpr int smem = 128 * 129 * 4;
-  auto kern = quant_tile_kernel<T, ROWS, TRANS>;
-  static std::atomic<uint64_t> done{0};
-  if (int rc = set_smem_limit_once(kern, smem, done, "cudaFuncSetAttribute(quantise)")) return rc;
-  const dim3 grid(static_cast<unsigned>((p.cols + 127) / 128), static_cast<unsigned>((p.rows + 127) / 128));
-  const cudaError_t e = launch_pdl(kern, grid, dim3(256), smem, s, p);
-  return e == cudaSuccess ? CHOREO_OK : cuda_fail(e, "quantise launch");
+template <typename Kern, typename... Args>
+int launch_quant(Kern kern, int64_t grid, int smem, std::atomic<uint64_t>& done, cudaStream_t s, Args... args) {
+  if (grid > INT32_MAX) return fail(CHOREO_ERR_UNSUPPORTED, "quantize: more than 2^31-1 tiles");
+  if (smem > 0)
+    if (int rc = set_smem_limit_once(kern, smem, done, "cudaFuncSetAttribute(quantize)")) return rc;
+  const cudaError_t e = launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(256), smem, s, args...);
+  return e == cudaSuccess ? CHOREO_OK : cuda_fail(e, "quantize launch");
+}
+
+template <typename T, int UNROLL>
+int launch_rows(const QuantParams& p, cudaStream_t s) {
+  constexpr int64_t span = UNROLL * 32 * Piece<T>::kElems;
+  const int64_t runs = (p.cols + span - 1) / span;
+  std::atomic<uint64_t> none{0};
+  return launch_quant(quant_rows_kernel<T, UNROLL>, (p.rows + 7) / 8 * runs, 0, none, s, p, runs);
+}
+
+template <typename T, bool SQUARE, bool TRANS>
+int launch_tile(const QuantParams& p, bool x_vec, cudaStream_t s) {
+  const int64_t grid = p.row_tiles * p.col_tiles;
+  if (!x_vec) {
+    static std::atomic<uint64_t> done{0};
+    return launch_quant(quant_unaligned_kernel<T, SQUARE, TRANS>, grid, 128 * 129 * 4, done, s, p);
+  }
+  if constexpr (SQUARE || TRANS) {
+    static std::atomic<uint64_t> done{0};
+    return launch_quant(quant_tile_kernel<T, SQUARE, TRANS>, grid, TRANS ? 128 * 128 * static_cast<int>(sizeof(T)) : 0,
+                        done, s, p);
+  } else {
+    // Four loads in flight a thread where that still leaves every SM two CTAs;
+    // a few rows are spread over as many SMs as one load each can reach.
+    const int64_t wide = (p.rows + 7) / 8 * ((p.cols + 128 * Piece<T>::kElems - 1) / (128 * Piece<T>::kElems));
+    return wide >= 2 * current_sm_count() ? launch_rows<T, 4>(p, s) : launch_rows<T, 1>(p, s);
+  }
 }
 
 template <typename T>
-int dispatch_quant(const QuantParams& p, bool rows, bool trans, cudaStream_t s) {
-  if (rows) return trans ? launch_quant<T, true, true>(p, s) : launch_quant<T, true, false>(p, s);
-  return trans ? launch_quant<T, false, true>(p, s) : launch_quant<T, false, false>(p, s);
+int dispatch_quant(const QuantParams& p, bool rows, bool trans, bool x_vec, cudaStream_t s) {
+  if (rows) return trans ? launch_tile<T, false, true>(p, x_vec, s) : launch_tile<T, false, false>(p, x_vec, s);
+  return trans ? launch_tile<T, true, true>(p, x_vec, s) : launch_tile<T, true, false>(p, x_vec, s);
 }
 
 }  // namespace
@@ -186,14 +491,17 @@ extern "C" int choreo_quantize_block(const choreo_quant_desc* d, void* stream) {
   p.scale = d->scale;
   p.scale_row = d->scale_row;
   p.scale_blk = d->scale_blk;
-  p.x_vec = ((reinterpret_cast<uintptr_t>(d->x) | static_cast<uintptr_t>(d->ldx * dtype_bytes(d->dtype))) & 15u) == 0;
-  p.q_vec = ((reinterpret_cast<uintptr_t>(d->q) | static_cast<uintptr_t>(d->ldq)) & 3u) == 0;
+  p.row_tiles = (p.rows + 127) / 128;
+  p.col_tiles = col_blocks;
+  const bool x_vec =
+      ((reinterpret_cast<uintptr_t>(d->x) | static_cast<uintptr_t>(d->ldx * dtype_bytes(d->dtype))) & 15u) == 0;
+  p.q_vec = ((reinterpret_cast<uintptr_t>(d->q) | static_cast<uintptr_t>(d->ldq)) & 7u) == 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool rows = d->block_rows == 1, trans = d->transpose != 0;
   switch (d->dtype) {
-    case CHOREO_DTYPE_F16: rc = dispatch_quant<__half>(p, rows, trans, s); break;
-    case CHOREO_DTYPE_BF16: rc = dispatch_quant<__nv_bfloat16>(p, rows, trans, s); break;
-    default: rc = dispatch_quant<float>(p, rows, trans, s); break;
+    case CHOREO_DTYPE_F16: rc = dispatch_quant<__half>(p, rows, trans, x_vec, s); break;
+    case CHOREO_DTYPE_BF16: rc = dispatch_quant<__nv_bfloat16>(p, rows, trans, x_vec, s); break;
+    default: rc = dispatch_quant<float>(p, rows, trans, x_vec, s); break;
   }
   return rc ? rc : ok();
 }
