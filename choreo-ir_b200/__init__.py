@@ -208,7 +208,7 @@ def dtype_code(t) -> int:
 def _stream_ptr(stream) -> int | None:
     if stream is None:
         import torch
-        return torch.cuda.current_stream().cuda_stream
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
     if isinstance(stream, int):
         return stream
     return stream.cuda_stream
@@ -453,13 +453,14 @@ _ACTS = {"silu": ACT_SILU, "gelu": ACT_GELU, "gelu_tanh": ACT_GELU_TANH, "relu":
 
 def _matrix(t, rows, cols, name, like=None):
     """A rows x cols torch matrix with contiguous rows; its leading dimension."""
-    if t.dim() != 2 or tuple(t.shape) != (rows, cols):
+    if t.shape != (rows, cols):
         raise ValueError(f"{name}: expected a {rows} x {cols} matrix, got {tuple(t.shape)}")
-    if t.stride(1) != 1 and cols > 1:
+    ld, inner = t.stride()
+    if inner != 1 and cols > 1:
         raise ValueError(f"{name}: innermost dimension must be contiguous")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
-        raise ValueError(f"{name}: dtype and device must be {like.dtype} on {like.device}")
-    return max(t.stride(0), cols) if rows == 1 else t.stride(0)
+    if like is not None and t.dtype != like.dtype:
+        raise ValueError(f"{name}: expected {like.dtype}, got {t.dtype}")
+    return ld if ld >= cols or rows > 1 else cols
 
 
 def _act_code(act):
@@ -478,24 +479,24 @@ def _workspace(need, workspace, device):
     return workspace, workspace.numel() * workspace.element_size()
 
 
+def _pair_ld(a, b, rows, cols, names, like):
+    """Leading dimension of two matrices that share one (both, or neither given)."""
+    ld = _matrix(a, rows, cols, names[0], like) if a is not None else 0
+    if b is not None:
+        ld_b = _matrix(b, rows, cols, names[1], like)
+        if a is not None and ld_b != ld:
+            raise ValueError(f"{names[0]} and {names[1]} must have the same row stride")
+    return ld
+
+
 def ffn_desc(x, w_gate, w_up, h, *, act="silu", trans_w=False, gate=None, up=None) -> FfnDesc:
-    d = FfnDesc()
-    d.m, d.k = x.shape
-    d.n = w_gate.shape[0] if trans_w else w_gate.shape[1]
-    wshape = (d.n, d.k) if trans_w else (d.k, d.n)
-    d.dtype, d.act, d.trans_w = dtype_code(x), _act_code(act), int(trans_w)
-    d.ldx = _matrix(x, d.m, d.k, "x")
-    d.ldw = _matrix(w_gate, *wshape, "w_gate", x)
-    if _matrix(w_up, *wshape, "w_up", x) != d.ldw:
-        raise ValueError("w_gate and w_up must have the same row stride")
-    d.ldh = _matrix(h, d.m, d.n, "h", x)
-    d.x, d.w_gate, d.w_up, d.h = _ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(h)
-    d.gate, d.up = _ptr(gate), _ptr(up)
-    if gate is not None:
-        d.ld_gu = _matrix(gate, d.m, d.n, "gate", x)
-    if up is not None and _matrix(up, d.m, d.n, "up", x) != d.ld_gu and gate is not None:
-        raise ValueError("gate and up must have the same row stride")
-    return d
+    m, k = x.shape
+    n = w_gate.shape[0] if trans_w else w_gate.shape[1]
+    wshape = (n, k) if trans_w else (k, n)
+    return FfnDesc(m, n, k, dtype_code(x), _act_code(act), x.data_ptr(), _matrix(x, m, k, "x"), w_gate.data_ptr(),
+                   w_up.data_ptr(), _pair_ld(w_gate, w_up, *wshape, ("w_gate", "w_up"), x), int(trans_w), 0,
+                   h.data_ptr(), _matrix(h, m, n, "h", x), _ptr(gate), _ptr(up),
+                   _pair_ld(gate, up, m, n, ("gate", "up"), x))
 
 
 def gated_ffn_query(d: FfnDesc) -> LaunchConfig:
@@ -513,41 +514,30 @@ def gated_ffn(x, w_gate, w_up, h, *, act="silu", trans_w=False, gate=None, up=No
     and up, when given, receive the two products for gated_ffn_backward. Rows
     may be padded. All are f16, or all bf16."""
     d = ffn_desc(x, w_gate, w_up, h, act=act, trans_w=trans_w, gate=gate, up=up)
+    stream = _stream_ptr(stream)
+    if workspace is None:
+        # aligned operands need none: ask for the size only when the call does
+        rc = lib.choreo_gated_ffn(C.byref(d), None, 0, stream)
+        if rc != ERR_WORKSPACE:
+            return check(rc)
     need = gated_ffn_query(d).workspace_bytes if workspace is None else 0
     workspace, ws_bytes = _workspace(need, workspace, h.device)
-    check(lib.choreo_gated_ffn(C.byref(d), _ptr(workspace), ws_bytes, _stream_ptr(stream)))
+    check(lib.choreo_gated_ffn(C.byref(d), _ptr(workspace), ws_bytes, stream))
 
 
 def ffn_grad_desc(dh, x, w_gate, w_up, *, dx=None, dw_gate=None, dw_up=None, gate=None, up=None, h=None, act="silu",
                   trans_w=False, accumulate=False) -> FfnGradDesc:
-    d = FfnGradDesc()
-    d.m, d.k = x.shape
-    d.n = dh.shape[1]
-    wshape = (d.n, d.k) if trans_w else (d.k, d.n)
-    d.dtype, d.act, d.trans_w = dtype_code(x), _act_code(act), int(trans_w)
-    d.ldx = _matrix(x, d.m, d.k, "x")
-    d.ldw = _matrix(w_gate, *wshape, "w_gate", x)
-    if _matrix(w_up, *wshape, "w_up", x) != d.ldw:
-        raise ValueError("w_gate and w_up must have the same row stride")
-    d.ld_dh = _matrix(dh, d.m, d.n, "dh", x)
-    d.x, d.w_gate, d.w_up, d.dh = _ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(dh)
-    d.gate, d.up, d.dx, d.dw_gate, d.dw_up, d.h = map(_ptr, (gate, up, dx, dw_gate, dw_up, h))
-    if gate is not None:
-        d.ld_gu = _matrix(gate, d.m, d.n, "gate", x)
-    if up is not None and _matrix(up, d.m, d.n, "up", x) != d.ld_gu and gate is not None:
-        raise ValueError("gate and up must have the same row stride")
-    if dx is not None:
-        d.ld_dx = _matrix(dx, d.m, d.k, "dx", x)
-    d.dtype_dw = d.dtype
-    if dw_gate is not None:
-        d.ld_dw = _matrix(dw_gate, *wshape, "dw_gate")
-        d.dtype_dw = dtype_code(dw_gate)
-    if dw_up is not None and _matrix(dw_up, *wshape, "dw_up", dw_gate) != d.ld_dw and dw_gate is not None:
-        raise ValueError("dw_gate and dw_up must have the same row stride")
-    if h is not None:
-        d.ldh = _matrix(h, d.m, d.n, "h", x)
-    d.accumulate_dw = int(accumulate)
-    return d
+    m, k = x.shape
+    n = dh.shape[1]
+    wshape = (n, k) if trans_w else (k, n)
+    code = dtype_code(x)
+    return FfnGradDesc(m, n, k, code, _act_code(act), x.data_ptr(), _matrix(x, m, k, "x"), w_gate.data_ptr(),
+                       w_up.data_ptr(), _pair_ld(w_gate, w_up, *wshape, ("w_gate", "w_up"), x), int(trans_w),
+                       dtype_code(dw_gate) if dw_gate is not None else code, dh.data_ptr(),
+                       _matrix(dh, m, n, "dh", x), _ptr(gate), _ptr(up), _pair_ld(gate, up, m, n, ("gate", "up"), x),
+                       _ptr(dx), _matrix(dx, m, k, "dx", x) if dx is not None else 0, _ptr(dw_gate), _ptr(dw_up),
+                       _pair_ld(dw_gate, dw_up, *wshape, ("dw_gate", "dw_up"), dw_gate), int(accumulate), 0, _ptr(h),
+                       _matrix(h, m, n, "h", x) if h is not None else 0)
 
 
 def gated_ffn_backward_query(d: FfnGradDesc) -> LaunchConfig:
@@ -571,16 +561,17 @@ def gated_ffn_backward(dh, x, w_gate, w_up, *, dx=None, dw_gate=None, dw_up=None
 
 def _e4m3_matrix(t, rows, cols, name):
     import torch
-    if t.dtype not in (torch.float8_e4m3fn, torch.uint8):
-        raise ValueError(f"{name}: e4m3 elements (torch.float8_e4m3fn or uint8) required, got {t.dtype}")
+    dt = t.dtype
+    if dt is not torch.float8_e4m3fn and dt is not torch.uint8:
+        raise ValueError(f"{name}: e4m3 elements (torch.float8_e4m3fn or uint8) required, got {dt}")
     return _matrix(t, rows, cols, name)
 
 
 def _scales(t, rows, blocks, name):
     import torch
-    if t.dtype != torch.float32 or tuple(t.shape) != (rows, blocks):
+    if t.dtype is not torch.float32 or t.shape != (rows, blocks):
         raise ValueError(f"{name}: expected f32 scales {rows} x {blocks}, got {t.dtype} {tuple(t.shape)}")
-    return t.stride(0), t.stride(1)
+    return t.stride()
 
 
 def quantize_block(x, q, scale, *, block_rows=1, transpose=False, stream=None) -> None:
@@ -591,37 +582,27 @@ def quantize_block(x, q, scale, *, block_rows=1, transpose=False, stream=None) -
     rows may be padded); scale is [row blocks, column blocks] with any positive
     strides. torch.empty(column blocks, row blocks).t() is the layout that
     gemm_block_scaled reads fastest."""
-    d = QuantDesc()
-    d.rows, d.cols = x.shape
-    r, c = (d.cols, d.rows) if transpose else (d.rows, d.cols)
-    d.dtype, d.transpose, d.block_rows = dtype_code(x), int(transpose), block_rows
-    d.ldx = _matrix(x, d.rows, d.cols, "x")
-    d.ldq = _e4m3_matrix(q, r, c, "q")
-    if block_rows in (1, 128):  # anything else is refused below
-        d.scale_row, d.scale_blk = _scales(scale, -(-r // block_rows), -(-c // 128), "scale")
-    d.x, d.q, d.scale = _ptr(x), _ptr(q), _ptr(scale)
+    rows, cols = x.shape
+    r, c = (cols, rows) if transpose else (rows, cols)
+    # another block_rows is refused by the library
+    strides = _scales(scale, -(-r // block_rows), -(-c // 128), "scale") if block_rows in (1, 128) else (1, 1)
+    d = QuantDesc(rows, cols, dtype_code(x), int(transpose), x.data_ptr(), _matrix(x, rows, cols, "x"), block_rows, 0,
+                  q.data_ptr(), _e4m3_matrix(q, r, c, "q"), scale.data_ptr(), *strides)
     check(lib.choreo_quantize_block(C.byref(d), _stream_ptr(stream)))
 
 
 def gemm_block_desc(a, scale_a, b, scale_b, c, *, alpha=1.0, beta=0.0, addend=None, bias=None,
                     relu=False) -> GemmBlockDesc:
-    d = GemmBlockDesc()
-    d.m, d.k = a.shape
-    d.n = b.shape[0]
-    blocks = -(-d.k // 128)
-    d.lda, d.ldb = _e4m3_matrix(a, d.m, d.k, "a"), _e4m3_matrix(b, d.n, d.k, "b")
-    d.scale_a_row, d.scale_a_blk = _scales(scale_a, d.m, blocks, "scale_a")
-    d.block_b = 1 if scale_b.dim() == 2 and scale_b.shape[0] == d.n else 128
-    d.scale_b_row, d.scale_b_blk = _scales(scale_b, -(-d.n // d.block_b), blocks, "scale_b")
-    d.ldc, d.dtype_c = _matrix(c, d.m, d.n, "c"), dtype_code(c)
-    d.a, d.scale_a, d.b, d.scale_b, d.c = map(_ptr, (a, scale_a, b, scale_b, c))
-    d.alpha, d.beta = alpha, beta
-    if addend is not None:
-        d.addend, d.ld_addend = _ptr(addend), _matrix(addend, d.m, d.n, "addend", c)
-    d.bias = _ptr(bias)
-    d.dtype_bias = dtype_code(bias) if bias is not None else F32
-    d.relu = int(relu)
-    return d
+    m, k = a.shape
+    n = b.shape[0]
+    blocks = -(-k // 128)
+    block_b = 1 if scale_b.shape[0] == n else 128
+    return GemmBlockDesc(m, n, k, a.data_ptr(), _e4m3_matrix(a, m, k, "a"), scale_a.data_ptr(),
+                         *_scales(scale_a, m, blocks, "scale_a"), b.data_ptr(), _e4m3_matrix(b, n, k, "b"),
+                         scale_b.data_ptr(), *_scales(scale_b, -(-n // block_b), blocks, "scale_b"), block_b,
+                         dtype_code(c), c.data_ptr(), _matrix(c, m, n, "c"), alpha, beta, _ptr(addend),
+                         _matrix(addend, m, n, "addend", c) if addend is not None else 0, _ptr(bias),
+                         dtype_code(bias) if bias is not None else F32, int(relu))
 
 
 def gemm_block_scaled_query(d: GemmBlockDesc) -> LaunchConfig:

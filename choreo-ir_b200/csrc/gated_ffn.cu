@@ -6,6 +6,7 @@
 #include "gated_ffn.cuh"
 #include "gated_ffn.h"
 #include "internal.h"
+#include "skinny.cuh"
 
 namespace choreo_impl {
 using namespace choreo_sm100;
@@ -102,7 +103,46 @@ TcConfig select_gate_config(int64_t m, int64_t n, int64_t k) {
       .cfg;
 }
 
+namespace {
+constexpr int kSkinnyCols = 64;  // columns of H in a skinny tile
+
+bool use_skinny(int64_t m, bool grad) { return m <= kSkinnyRows && !grad; }
+
+int launch_gate_skinny(const GateProblem& p, cudaStream_t stream) {
+  CUtensorMap tx;
+  TwoMaps tw;
+  int rc = encode_matrix(&tx, p.bf16, p.x, p.m, p.k, p.ldx, 64, static_cast<uint32_t>(skinny_tokens(p.m)));
+  if (rc) return rc;
+  for (int i = 0; i < 2; ++i) {
+    const void* w = i == 0 ? p.w_gate : p.w_up;
+    rc = p.w_mn ? encode_matrix(&tw.m[i], p.bf16, w, p.k, p.n, p.ldw, 64, 64)
+                : encode_matrix(&tw.m[i], p.bf16, w, p.n, p.k, p.ldw, 64, 64);
+    if (rc) return rc;
+  }
+  SkinnyParams kp;
+  std::memset(&kp, 0, sizeof(kp));
+  kp.m = static_cast<int32_t>(p.m);
+  kp.n = static_cast<int32_t>(p.n);
+  kp.num_k_blocks = static_cast<int32_t>((p.k + kBK - 1) / kBK);
+  const int64_t tiles = (p.n + kSkinnyCols - 1) / kSkinnyCols;
+  kp.split = skinny_split(tiles, kp.num_k_blocks, current_sm_count());
+  kp.ab_bf16 = p.bf16 ? 1 : 0;
+  kp.act = p.act;
+  kp.c = p.h;
+  kp.ldc = p.ldh;
+  kp.out1 = p.out1;
+  kp.out2 = p.out2;
+  kp.ld12 = p.ld12;
+  kp.status = status_word();
+  kp.timeout_ns = wait_timeout_ns();
+  if (kp.status == nullptr) return CHOREO_ERR_CUDA;
+  return p.w_mn ? launch_skinny<kGateCols>(tw, tx, kp, tiles, stream)
+                : launch_skinny<kGateRows>(tw, tx, kp, tiles, stream);
+}
+}  // namespace
+
 int launch_gate_tiles(const GateProblem& p, cudaStream_t stream) {
+  if (use_skinny(p.m, p.dh != nullptr)) return launch_gate_skinny(p, stream);
   const TcConfig cfg = select_gate_config(p.m, p.n, p.k);
   CUtensorMap ta;
   TwoMaps tb;
@@ -245,25 +285,42 @@ int choreo_gated_ffn_query(const choreo_ffn_desc* d, choreo_launch_config* out) 
   if (rc) return rc;
   if (out == nullptr) return fail(CHOREO_ERR_INVALID_ARG, "gated FFN query: null output");
   std::memset(out, 0, sizeof(*out));
-  const TcConfig c = select_gate_config(d->m, d->n, d->k);
-  out->kernel = 4;
-  out->tile_m = tile_rows_of(c);
-  out->tile_n = c.bn / 2;
-  out->tile_k = kBK;
-  out->stages = c.stages;
-  out->cluster_m = c.pair ? 2 : 1;
-  out->tiles = ((d->m + out->tile_m - 1) / out->tile_m) * ((d->n + out->tile_n - 1) / out->tile_n);
   const int sms = current_sm_count();
-  out->grid_x = static_cast<int32_t>(c.pair ? 2 * std::min<int64_t>(out->tiles, sms / 2)
-                                            : std::min<int64_t>(out->tiles, sms));
+  out->kernel = 4;
   out->grid_y = out->grid_z = 1;
-  out->block_x = kTcThreads;
-  out->smem_bytes = c.smem;
-  out->tmem_cols = c.wide ? 512 : 2 * c.bn;
+  out->tile_k = kBK;
+  out->split_k = 1;
   FfnOperands o;
   plan_ffn_operands(&o, d->x, d->ldx, d->w_gate, d->w_up, d->ldw, d->trans_w != 0, d->m, d->n, d->k);
   out->workspace_bytes = out->workspace_min_bytes = o.bytes;
-  out->split_k = 1;
+  if (use_skinny(d->m, false)) {
+    const int nt = skinny_tokens(d->m);
+    out->tile_m = nt;
+    out->tile_n = kSkinnyCols;
+    out->tiles = (d->n + kSkinnyCols - 1) / kSkinnyCols;
+    out->split_k = skinny_split(out->tiles, (d->k + kBK - 1) / kBK, sms);
+    out->cluster_m = static_cast<int32_t>(out->split_k);
+    out->tiles *= out->split_k;
+    out->grid_x = static_cast<int32_t>(out->tiles);
+    out->block_x = kSkinnyThreads;
+    out->stages = nt == 16 ? SkinnyShape<16>::kStages : nt == 32 ? SkinnyShape<32>::kStages
+                : nt == 64 ? SkinnyShape<64>::kStages : SkinnyShape<128>::kStages;
+    out->smem_bytes = nt == 16 ? SkinnyShape<16>::kSmem : nt == 32 ? SkinnyShape<32>::kSmem
+                    : nt == 64 ? SkinnyShape<64>::kSmem : SkinnyShape<128>::kSmem;
+    out->tmem_cols = std::max(nt, 32);
+    return ok();
+  }
+  const TcConfig c = select_gate_config(d->m, d->n, d->k);
+  out->tile_m = tile_rows_of(c);
+  out->tile_n = c.bn / 2;
+  out->stages = c.stages;
+  out->cluster_m = c.pair ? 2 : 1;
+  out->tiles = ((d->m + out->tile_m - 1) / out->tile_m) * ((d->n + out->tile_n - 1) / out->tile_n);
+  out->grid_x = static_cast<int32_t>(c.pair ? 2 * std::min<int64_t>(out->tiles, sms / 2)
+                                            : std::min<int64_t>(out->tiles, sms));
+  out->block_x = kTcThreads;
+  out->smem_bytes = c.smem;
+  out->tmem_cols = c.wide ? 512 : 2 * c.bn;
   return ok();
 }
 

@@ -15,6 +15,7 @@
 #include <cstdlib>
 
 #include "internal.h"
+#include "skinny.cuh"
 #include "tc_kernel.cuh"
 
 namespace choreo_sm100 {
@@ -66,14 +67,6 @@ __device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
   return r;
 }
-// A load the compiler leaves where it is written: ahead of a wait, not next to
-// the use of its value.
-__device__ __forceinline__ float ldg_early(const float* p) {
-  float v;
-  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
-  return v;
-}
-
 // d += (a0, a1) * s on packed pairs, one rounding per element.
 __device__ __forceinline__ void fma2_acc(uint64_t& d, uint32_t a0, uint32_t a1, uint64_t s) {
   uint64_t a;
@@ -555,6 +548,45 @@ int block_grid(int64_t tiles, const BlockConfig& c) {
   return static_cast<int>(c.pair ? 2 * std::min<int64_t>(tiles, sms / 2) : std::min<int64_t>(tiles, sms));
 }
 
+constexpr int kSkinnyCols = 128;  // columns of C in a skinny tile
+
+int launch_block_skinny(const choreo_gemm_block_desc& d, cudaStream_t stream) {
+  CUtensorMap tx;
+  TwoMaps tw;
+  int rc = encode_e4m3(&tx, d.a, d.m, d.k, d.lda, static_cast<uint32_t>(skinny_tokens(d.m)));
+  if (rc) return rc;
+  if ((rc = encode_e4m3(&tw.m[0], d.b, d.n, d.k, d.ldb, 128))) return rc;
+  tw.m[1] = tw.m[0];
+  SkinnyParams kp;
+  std::memset(&kp, 0, sizeof(kp));
+  kp.m = static_cast<int32_t>(d.m);
+  kp.n = static_cast<int32_t>(d.n);
+  kp.num_k_blocks = static_cast<int32_t>((d.k + kBlockK - 1) / kBlockK);
+  const int64_t tiles = (d.n + kSkinnyCols - 1) / kSkinnyCols;
+  kp.split = skinny_split(tiles, kp.num_k_blocks, current_sm_count());
+  kp.c = d.c;
+  kp.ldc = d.ldc;
+  kp.alpha = d.alpha;
+  kp.beta = d.beta;
+  kp.bias = d.bias;
+  kp.dtype_bias = d.dtype_bias;
+  kp.relu = d.relu;
+  kp.dtype_c = d.dtype_c;
+  kp.block_b = d.block_b;
+  kp.sa = d.scale_a;
+  kp.sa_row = d.scale_a_row;
+  kp.sa_blk = d.scale_a_blk;
+  kp.sb = d.scale_b;
+  kp.sb_row = d.scale_b_row;
+  kp.sb_blk = d.scale_b_blk;
+  kp.d = d.addend ? d.addend : d.c;
+  kp.ldd = d.addend ? d.ld_addend : d.ldc;
+  kp.status = status_word();
+  kp.timeout_ns = wait_timeout_ns();
+  if (kp.status == nullptr) return CHOREO_ERR_CUDA;
+  return launch_skinny<kBlock>(tw, tx, kp, tiles, stream);
+}
+
 }  // namespace
 }  // namespace choreo_impl
 
@@ -567,26 +599,47 @@ int choreo_gemm_block_scaled_query(const choreo_gemm_block_desc* d, choreo_launc
   if (rc) return rc;
   if (out == nullptr) return fail(CHOREO_ERR_INVALID_ARG, "block-scaled GEMM query: null output");
   std::memset(out, 0, sizeof(*out));
-  const BlockConfig c = select_block_config(d->m, d->n);
   out->kernel = 5;
+  out->tile_k = kBlockK;
+  out->grid_y = out->grid_z = 1;
+  out->split_k = 1;
+  if (d->m <= kSkinnyRows) {
+    const int nt = skinny_tokens(d->m);
+    out->tile_m = nt;
+    out->tile_n = kSkinnyCols;
+    out->tiles = (d->n + kSkinnyCols - 1) / kSkinnyCols;
+    out->split_k = skinny_split(out->tiles, (d->k + kBlockK - 1) / kBlockK, current_sm_count());
+    out->cluster_m = static_cast<int32_t>(out->split_k);
+    out->tiles *= out->split_k;
+    out->grid_x = static_cast<int32_t>(out->tiles);
+    out->block_x = kSkinnyThreads;
+    out->stages = nt == 16 ? SkinnyShape<16>::kStages : nt == 32 ? SkinnyShape<32>::kStages
+                : nt == 64 ? SkinnyShape<64>::kStages : SkinnyShape<128>::kStages;
+    out->smem_bytes = nt == 16 ? SkinnyShape<16>::kSmem : nt == 32 ? SkinnyShape<32>::kSmem
+                    : nt == 64 ? SkinnyShape<64>::kSmem : SkinnyShape<128>::kSmem;
+    out->tmem_cols = nt * (nt <= 64 ? 4 : 2);
+    return ok();
+  }
+  const BlockConfig c = select_block_config(d->m, d->n);
   out->tile_m = c.pair ? 256 : 128;
   out->tile_n = c.bn;
-  out->tile_k = kBlockK;
   out->stages = BlockShape<true, 256>::kStages;
   out->cluster_m = c.pair ? 2 : 1;
   out->tiles = block_tiles(*d, c);
   out->grid_x = block_grid(out->tiles, c);
-  out->grid_y = out->grid_z = 1;
   out->block_x = kBlockThreads;
   out->smem_bytes = c.pair ? BlockShape<true, 256>::kSmem : BlockShape<false, 128>::kSmem;
   out->tmem_cols = 512;
-  out->split_k = 1;
   return ok();
 }
 
 int choreo_gemm_block_scaled(const choreo_gemm_block_desc* d, void* stream) {
   int rc = validate_block(d);
   if (rc) return rc;
+  if (d->m <= kSkinnyRows) {
+    rc = launch_block_skinny(*d, static_cast<cudaStream_t>(stream));
+    return rc ? rc : ok();
+  }
   const BlockConfig c = select_block_config(d->m, d->n);
   CUtensorMap ta, tb, tc;
   if ((rc = encode_e4m3(&ta, d->a, d->m, d->k, d->lda, 128))) return rc;

@@ -420,6 +420,14 @@ __host__ __device__ constexpr uint32_t idesc_e4m3(int m, int n) {
   return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+// A load the compiler leaves where it is written: ahead of a wait, not next to
+// the use of its value.
+__device__ __forceinline__ float ldg_early(const float* p) {
+  float v;
+  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+
 // Moves registers between warpgroups: every warp of the warpgroup executes it.
 template <int REGS>
 __device__ __forceinline__ void regs_inc() {
