@@ -23,10 +23,34 @@ namespace choreo_sm100 {
 // ------------------------------------------------------------------ activation
 // Value and slope of the gate activation. exp through __expf (2 ulp near 0,
 // relative error ~ |g| 2^-24 beyond): far below the 16-bit outputs' rounding.
+
+// The normal distribution function, through erfc(x) = t exp(P(t) - x^2),
+// t = 1 / (1 + x / 2): a Chebyshev fit of degree 9 of the logarithm (the form
+// of Press et al., Numerical Recipes, "Error Function"), fitted in 64 bits to
+// 1.0e-7. No branch and no cancellation in the lower tail: relative error below
+// 2e-6 for g > -4 and 2e-5 for g > -12 in fp32, against 2^-12 (fp16) of the
+// outputs' rounding.
+__device__ __forceinline__ float normal_cdf(float g) {
+  const float a = fabsf(g) * 0.7071067811865476f;
+  const float t = __fdividef(1.f, fmaf(0.5f, a, 1.f));
+  float q = 0.1708727777f;
+  q = fmaf(q, t, -0.8221522570f);
+  q = fmaf(q, t, 1.488515854f);
+  q = fmaf(q, t, -1.135203958f);
+  q = fmaf(q, t, 0.2788680792f);
+  q = fmaf(q, t, -0.1862880588f);
+  q = fmaf(q, t, 0.09678418934f);
+  q = fmaf(q, t, 0.3740919530f);
+  q = fmaf(q, t, 1.000023723f);
+  q = fmaf(q, t, -1.265512228f);
+  const float half_erfc = 0.5f * t * __expf(fmaf(-a, a, q));
+  return g < 0.f ? half_erfc : 1.f - half_erfc;
+}
+
 template <int ACT>
 __device__ __forceinline__ float act_value(float g) {
   if constexpr (ACT == CHOREO_ACT_SILU) return __fdividef(g, 1.f + __expf(-g));
-  if constexpr (ACT == CHOREO_ACT_GELU) return g * normcdff(g);
+  if constexpr (ACT == CHOREO_ACT_GELU) return g * normal_cdf(g);
   if constexpr (ACT == CHOREO_ACT_GELU_TANH) {
     // (1 + tanh z) / 2 = 1 / (1 + exp(-2 z))
     const float z2 = 1.5957691216057308f * g * fmaf(0.044715f * g, g, 1.f);
@@ -41,7 +65,7 @@ __device__ __forceinline__ void act_value_slope(float g, float& v, float& dv) {
     v = g * s;
     dv = fmaf(v, 1.f - s, s);
   } else if constexpr (ACT == CHOREO_ACT_GELU) {
-    const float phi = normcdff(g);
+    const float phi = normal_cdf(g);
     v = g * phi;
     dv = fmaf(g * 0.3989422804014327f, __expf(-0.5f * g * g), phi);
   } else if constexpr (ACT == CHOREO_ACT_GELU_TANH) {

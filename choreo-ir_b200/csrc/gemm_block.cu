@@ -12,7 +12,6 @@
 
 #include <algorithm>
 #include <cstring>
-#include <cstdlib>
 
 #include "internal.h"
 #include "skinny.cuh"
@@ -38,6 +37,8 @@ struct alignas(8) BlockBarriers {
   uint64_t full[STAGES];      // the stage's tiles have landed
   uint64_t empty[STAGES];     // its MMAs are done: the stage is free, its block's accumulator is full
   uint64_t tmem_empty[BUFS];  // the epilogue has read the accumulator
+  uint64_t scale_full[4];     // a block's scales are in their slot
+  uint64_t scale_empty[4];    // the epilogue has read them
   uint64_t drain;
   uint64_t probe[2];
   uint32_t tmem_base;
@@ -49,11 +50,14 @@ struct BlockShape {
   static constexpr int kBRows = PAIR ? BN / 2 : BN;  // B rows one CTA stages
   static constexpr uint32_t kAStage = kBM * kBlockK;
   static constexpr uint32_t kBStage = kBRows * kBlockK;
-  static constexpr int kStages = (PAIR ? BN / 2 : BN) == 256 ? 4 : (PAIR && BN == 128 ? 8 : 6);
+  static constexpr int kStages = 6;
   static constexpr int kBufs = 512 / BN;  // block accumulators in TMEM
   using Barriers = BlockBarriers<kStages, kBufs>;
-  static constexpr int kSmem = kStages * static_cast<int>(kAStage + kBStage) + kStagingBytes + 1024 +
-                               static_cast<int>(sizeof(Barriers));
+  static constexpr uint32_t kStaging = kEpiWarps * 2048;             // 32 rows x 64 bytes a warp
+  static constexpr int kSlots = 4;                                   // scale slots
+  static constexpr uint32_t kSlotFloats = 128 + (BN > 128 ? BN : 128);  // rows', then columns' (see the scale warps)
+  static constexpr int kSmem = kStages * static_cast<int>(kAStage + kBStage) + static_cast<int>(kStaging) +
+                               kSlots * static_cast<int>(kSlotFloats) * 4 + 1024 + static_cast<int>(sizeof(Barriers));
   // 128 sums a thread and two 32-column reads in flight need more registers
   // than an even share of the SM's
   static constexpr bool kMoveRegs = BN == 256;
@@ -78,57 +82,72 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+__device__ __forceinline__ float ld_shared_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
 __device__ __forceinline__ void ld_shared_2x64(uint32_t addr, uint64_t& a, uint64_t& b) {
   asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(a), "=l"(b) : "r"(addr));
 }
 
-// Writes one warp's 32 rows x kCols columns of sums.
+// Writes one warp's 32 rows x kCols columns of sums, 32 columns at a time:
+// through its 2 KB staging buffer (32 rows of 64 bytes in the 64-byte swizzle:
+// 16-byte chunk j of row r at j ^ (r / 2 % 4)) and bulk tensor stores, or
+// element by element where those are not legal.
 template <int kCols, typename OutT>
 __device__ __forceinline__ void block_output(const uint64_t (&acc)[kCols / 2], int n_first, int row0, const BlockParams& p,
                                              const CUtensorMap* tma_c, uint32_t stage_buf, int lane) {
-  constexpr int E = 128 / static_cast<int>(sizeof(OutT));  // columns per 128-byte staging row
-  constexpr int kCpg = E / 32;
+  constexpr int E = 64 / static_cast<int>(sizeof(OutT));  // columns per staging row
   const int row = row0 + lane;
   const bool row_ok = row < p.m;
   const OutT* drow = static_cast<const OutT*>(p.d) + static_cast<int64_t>(row_ok ? row : 0) * p.ldd;
   OutT* crow = static_cast<OutT*>(p.c) + static_cast<int64_t>(row_ok ? row : 0) * p.ldc;
   TcParams pd = p;
   pd.c_vec_ok = p.d_vec;
+  const uint32_t row_addr = stage_buf + static_cast<uint32_t>(lane) * 64u;
+  const int sw = (lane >> 1) & 3;
 #pragma unroll
-  for (int g = 0; g < kCols / E; ++g) {
-    const int n_base = n_first + g * E;
+  for (int c = 0; c < kCols / 32; ++c) {
+    const int n_base = n_first + c * 32;
     if (n_base >= p.n) break;  // warp-uniform
+    uint32_t r[32];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      asm("mov.b64 {%0, %1}, %2;" : "=r"(r[2 * i]), "=r"(r[2 * i + 1]) : "l"(acc[c * 16 + i]));
+    float v[32];
+    epilogue_values<OutT>(r, v, drow, n_base, pd, row_ok, lane);
     // A bulk tensor store clips columns in whole 16 bytes: a ragged last group
     // that ends inside 16 bytes is stored element by element.
-    const bool tma = p.c_tma != 0 && (n_base + E <= p.n || p.n * static_cast<int>(sizeof(OutT)) % 16 == 0);
-    if (tma) {
-      if (lane == 0) bulk_wait_read_all();  // the warp's previous store has read the buffer
-      __syncwarp();
-    }
+    if (p.c_tma != 0 && (n_base + 32 <= p.n || p.n * static_cast<int>(sizeof(OutT)) % 16 == 0)) {
 #pragma unroll
-    for (int c = 0; c < kCpg; ++c) {
-      uint32_t r[32];
+      for (int g = 0; g < 32 / E; ++g) {
+        if (n_base + g * E >= p.n) break;  // warp-uniform
+        if (lane == 0) bulk_wait_read_all();  // the warp's previous store has read the buffer
+        __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        asm("mov.b64 {%0, %1}, %2;" : "=r"(r[2 * i]), "=r"(r[2 * i + 1]) : "l"(acc[(g * E + c * 32) / 2 + i]));
-      float v[32];
-      epilogue_values<OutT>(r, v, drow, n_base + c * 32, pd, row_ok, lane);
-      if (tma) {
-        stage_row_32<OutT>(v, stage_buf + static_cast<uint32_t>(lane) * 128u, lane,
-                           c * (32 * static_cast<int>(sizeof(OutT)) / 16));
-      } else if (row_ok) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (n_base + c * 32 + i < p.n) crow[n_base + c * 32 + i] = from_f32<OutT>(v[i]);
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t at = row_addr + static_cast<uint32_t>((j ^ sw) << 4);
+          if constexpr (sizeof(OutT) == 2)
+            st_shared_v4(at, pack2(v[8 * j], v[8 * j + 1], static_cast<OutT*>(nullptr)),
+                         pack2(v[8 * j + 2], v[8 * j + 3], static_cast<OutT*>(nullptr)),
+                         pack2(v[8 * j + 4], v[8 * j + 5], static_cast<OutT*>(nullptr)),
+                         pack2(v[8 * j + 6], v[8 * j + 7], static_cast<OutT*>(nullptr)));
+          else
+            st_shared_v4(at, __float_as_uint(v[g * 16 + 4 * j]), __float_as_uint(v[g * 16 + 4 * j + 1]),
+                         __float_as_uint(v[g * 16 + 4 * j + 2]), __float_as_uint(v[g * 16 + 4 * j + 3]));
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_3d(tma_c, stage_buf, n_base + g * E, row0, 0);
+          bulk_commit_group();
+        }
       }
-    }
-    if (tma) {
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        tma_store_3d(tma_c, stage_buf, n_base, row0, 0);
-        bulk_commit_group();
-      }
+    } else if (row_ok) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (n_base + i < p.n) crow[n_base + i] = from_f32<OutT>(v[i]);
     }
   }
 }
@@ -140,7 +159,6 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
   using S = BlockShape<PAIR, BN>;
   constexpr int STAGES = S::kStages;
   constexpr int kCols = BN / 2;  // columns of one epilogue warp
-  constexpr int kAhead = 1;
   constexpr uint32_t kTmemCols = 512;
   constexpr int kBufs = S::kBufs;
   extern __shared__ uint8_t smem_raw[];
@@ -149,7 +167,8 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
   uint8_t* s_a = smem;
   uint8_t* s_b = smem + STAGES * S::kAStage;
   uint8_t* s_stage = s_b + STAGES * S::kBStage;
-  auto* bars = reinterpret_cast<typename S::Barriers*>(s_stage + kStagingBytes);
+  float* s_scale = reinterpret_cast<float*>(s_stage + S::kStaging);
+  auto* bars = reinterpret_cast<typename S::Barriers*>(s_scale + S::kSlots * S::kSlotFloats);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0;
@@ -165,6 +184,10 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
     }
     for (int i = 0; i < kBufs; ++i) {
       mbar_init(smem_u32(&bars->tmem_empty[i]), (PAIR ? 2 : 1) * kEpiWarps);
+    }
+    for (int i = 0; i < S::kSlots; ++i) {
+      mbar_init(smem_u32(&bars->scale_full[i]), 2);
+      mbar_init(smem_u32(&bars->scale_empty[i]), kEpiWarps);
     }
     mbar_init(smem_u32(&bars->drain), 1);
     bars->abort = 0;
@@ -249,9 +272,7 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
       uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 1;
       const int64_t blocks = (p.num_tiles - first + step - 1) / step * p.num_k_blocks;
       for (int64_t i = 0; i < blocks; ++i) {
-        const bool ready = mbar_wait(bar_full + 8 * stage, phase, wctx, kStatusTimeoutMma) &&
-                           mbar_wait(bar_free + 8 * buf, buf_phase, wctx, kStatusTimeoutMma);
-        if (!__all_sync(0xffffffffu, ready)) break;
+        if (!mbar_wait_warp2(bar_full + 8 * stage, phase, bar_free + 8 * buf, buf_phase, wctx, kStatusTimeoutMma)) break;
         tc_fence_after();
         const uint64_t ad = smem_desc_advance(desc_a, stage * S::kAStage);
         const uint64_t bd = smem_desc_advance(desc_b, stage * S::kBStage);
@@ -275,18 +296,95 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
       }
       mbar_wait(smem_u32(&bars->drain), 0, wctx, kStatusTimeoutDrain, false);
       __syncwarp();
+    } else if (warp >= 2) {
+      // ------------------------------------------------------- scale warps
+      // Each k-block's scales go through a ring of shared-memory slots, so the
+      // epilogue neither addresses nor waits for global memory: with one scale
+      // per 128 rows of B the products sa(row) sb(column half), 2 x 128; else
+      // the 128 row scales and the BN column scales. The two warps take half
+      // of the rows and of the columns each, loaded kAhead blocks ahead.
+      griddep_wait();
+      constexpr int kAhead = 4;
+      constexpr int kSb = BVEC ? BN / 64 : 2;  // column values a lane holds
+      const int half = warp - 2;
+      uint32_t slot = 0, phase = 0;
+      bool ok = true;
+      for (int64_t t = first; t < p.num_tiles && ok; t += step) {
+        int b, mb, nb;
+        tile_coords(t, p, b, mb, nb);
+        const int r0 = mb * kTileM + static_cast<int>(rank) * kBM + half * 64 + lane;
+        const float* sa[2];
+        const float* sb[kSb];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) sa[i] = p.sa + static_cast<int64_t>(min(r0 + 32 * i, p.m - 1)) * p.sa_row;
+#pragma unroll
+        for (int i = 0; i < kSb; ++i) {
+          const int n = BVEC ? nb * BN + half * (BN / 2) + 32 * i + lane : nb * BN + i * (BN / 2);
+          sb[i] = p.sb + static_cast<int64_t>(min(n, p.n - 1) / (BVEC ? 1 : 128)) * p.sb_row;
+        }
+        float qa[kAhead][2], qb[kAhead][kSb];
+        auto load = [&](int kb, float (&va)[2], float (&vb)[kSb]) {
+          if (kb >= p.num_k_blocks) return;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            va[i] = ldg_early(sa[i]);
+            sa[i] += p.sa_blk;
+          }
+#pragma unroll
+          for (int i = 0; i < kSb; ++i) {
+            vb[i] = ldg_early(sb[i]);
+            sb[i] += p.sb_blk;
+          }
+        };
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) load(i, qa[i], qb[i]);
+        // Unrolled by kAhead: each queue entry is registers of its own (moving
+        // a value that is still in flight would wait for it).
+#pragma unroll 1
+        for (int kb0 = 0; kb0 < p.num_k_blocks && ok; kb0 += kAhead) {
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {
+            if (kb0 + u >= p.num_k_blocks) break;
+            if (!mbar_wait_warp(smem_u32(&bars->scale_empty[slot]), phase ^ 1, wctx, kStatusTimeoutProducer)) {
+              ok = false;
+              break;
+            }
+            float* rows = s_scale + slot * S::kSlotFloats + half * 64 + lane;
+            if constexpr (BVEC) {
+              float* cols = s_scale + slot * S::kSlotFloats + 128 + half * (BN / 2) + lane;
+#pragma unroll
+              for (int i = 0; i < 2; ++i) rows[32 * i] = qa[u][i];
+#pragma unroll
+              for (int i = 0; i < kSb; ++i) cols[32 * i] = qb[u][i];
+            } else {
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) rows[h * 128 + 32 * i] = qa[u][i] * qb[u][h];
+            }
+            __syncwarp();
+            mbar_arrive_lane0(smem_u32(&bars->scale_full[slot]), lane);
+            load(kb0 + u + kAhead, qa[u], qb[u]);
+            if (++slot == S::kSlots) { slot = 0; phase ^= 1; }
+          }
+        }
+      }
     }
   } else {
     if constexpr (S::kMoveRegs) regs_inc<S::kEpiRegs>();
     // ------------------------------------------------------------ epilogue
     const int quarter = warp & 3;
     const int col_half = (warp - 4) >> 2;
-    const uint32_t stage_buf = smem_u32(s_stage) + static_cast<uint32_t>(warp - 4) * 4096u;
+    const uint32_t stage_buf = smem_u32(s_stage) + static_cast<uint32_t>(warp - 4) * 2048u;
     const uint32_t tmem_warp = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + col_half * kCols;
     const uint32_t bar_done = smem_u32(&bars->empty[0]);
     const uint32_t bar_free = PAIR ? mapa_shared(smem_u32(&bars->tmem_empty[0]), 0) : smem_u32(&bars->tmem_empty[0]);
+    const uint32_t scale_full = smem_u32(&bars->scale_full[0]), scale_empty = smem_u32(&bars->scale_empty[0]);
+    // this lane's row scale, and the warp's column scales, in slot 0
+    const uint32_t scale_row = smem_u32(s_scale) + static_cast<uint32_t>((BVEC ? 0 : col_half * 128) + quarter * 32 + lane) * 4u;
+    const uint32_t scale_col = smem_u32(s_scale) + static_cast<uint32_t>(128 + col_half * kCols) * 4u;
     griddep_wait();
-    uint32_t stage = 0, phase = 0, buf = 0;
+    uint32_t stage = 0, phase = 0, buf = 0, slot = 0, slot_phase = 0;
     bool ok = true;
     for (int64_t t = first; t < p.num_tiles && ok; t += step) {
       int b, mb, nb;
@@ -294,108 +392,59 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
       const int row0 = mb * kTileM + static_cast<int>(rank) * kBM + quarter * 32;
       const int n_first = nb * BN + col_half * kCols;
       const bool active = row0 < p.m && n_first < p.n;
-      const int row = min(row0 + lane, p.m - 1);
-      const float* sa = p.sa + static_cast<int64_t>(row) * p.sa_row;
-      // BVEC: lane l holds the scales of columns n_first + 32 c + l
-      const float* sb[BVEC ? kCols / 32 : 1];
-      if constexpr (BVEC) {
-#pragma unroll
-        for (int c = 0; c < kCols / 32; ++c)
-          sb[c] = p.sb + static_cast<int64_t>(min(n_first + 32 * c + lane, p.n - 1)) * p.sb_row;
-      } else {
-        sb[0] = p.sb + static_cast<int64_t>(min(n_first, p.n - 1) / 128) * p.sb_row;
-      }
       uint64_t acc[kCols / 2];  // the warp's sums, in pairs of columns
 #pragma unroll
       for (int i = 0; i < kCols / 2; ++i) acc[i] = 0;
-      // Scales are loaded kAhead k-blocks before their use: one k-block takes
-      // less time than a load from L2 or HBM.
-      constexpr int kSb = BVEC ? kCols / 32 : 1;
-      float ahead_a[kAhead], ahead_b[kAhead][kSb];
-      auto load_scales = [&](int kb, float& a, float (&bv)[kSb]) {
-        if (kb >= p.num_k_blocks) return;
-        a = ldg_early(sa);
-        sa += p.sa_blk;
-#pragma unroll
-        for (int c = 0; c < kSb; ++c) {
-          bv[c] = ldg_early(sb[c]);
-          sb[c] += p.sb_blk;
-        }
-      };
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) load_scales(i, ahead_a[i], ahead_b[i]);
-      if constexpr (BVEC) {
-        if (lane == 0) bulk_wait_read_all();  // the previous tile's stores have read the buffer
-        __syncwarp();
-      }
-      // Unrolled by kAhead so that each slot of the scale queue is a register
-      // of its own (moving a value that is still in flight would wait for it).
 #pragma unroll 1
-      for (int kb0 = 0; kb0 < p.num_k_blocks && ok; kb0 += kAhead) {
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int kb = kb0 + u;
-        if (kb >= p.num_k_blocks) break;
-        const float cur_a = ahead_a[u];
-        float s = 0.f;
-        uint32_t sbuf = 0;
-        if constexpr (BVEC) {
-          // the block's column scales, read back below as broadcasts
-          sbuf = stage_buf + (kb & 1) * 512u;
-#pragma unroll
-          for (int c = 0; c < kSb; ++c) st_shared_f32(sbuf + static_cast<uint32_t>(c * 32 + lane) * 4u, ahead_b[u][c]);
-          __syncwarp();
-        } else {
-          s = cur_a * ahead_b[u][0];
-        }
-        load_scales(kb + kAhead, ahead_a[u], ahead_b[u]);
-        const bool ready = mbar_wait(bar_done + 8 * stage, phase, wctx, kStatusTimeoutEpilogue);
-        if (!__all_sync(0xffffffffu, ready)) {
+      for (int kb = 0; kb < p.num_k_blocks; ++kb) {
+        if (!mbar_wait_warp2(scale_full + 8 * slot, slot_phase, bar_done + 8 * stage, phase, wctx,
+                             kStatusTimeoutEpilogue)) {
           ok = false;
           break;
         }
         tc_fence_after();
         const uint32_t taddr = tmem_warp + buf * BN;
-        const uint32_t free_bar = bar_free + 8 * buf;
-        if (++stage == STAGES) { stage = 0; phase ^= 1; }
-        if (++buf == kBufs) buf = 0;
+        // Two 32-column reads of TMEM alternate: one is in flight while the
+        // other is used. Warps past the matrix's edge add up zeros rather than
+        // branch: without branches the warp stays converged and the chunks in
+        // one piece of code (8192^3: 866 -> 848 cycles a k-block, with column
+        // scales 1559 -> 1342).
+        uint32_t r[2][32];
+        tmem_ld_32x32b_x32(taddr, r[0]);
+        const float s = ld_shared_f32(scale_row + slot * (S::kSlotFloats * 4));
+        const uint32_t cols = scale_col + slot * (S::kSlotFloats * 4);
+        const uint64_t s2 = pack_f32x2(s, s);
         auto release = [&] {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) {
-            if constexpr (PAIR) mbar_arrive_cluster(free_bar); else mbar_arrive(free_bar);
-          }
+          if constexpr (PAIR)
+            mbar_arrive_cluster_lane0(bar_free + 8 * buf, lane);
+          else
+            mbar_arrive_lane0(bar_free + 8 * buf, lane);
         };
-        if (!active) {
-          release();
-          continue;
-        }
-        // One 32-column read at a time: the SM sub-partition's other epilogue
-        // warp works meanwhile, and a second one in flight would not fit the
-        // registers beside the sums.
+        tmem_wait_ld(r[0]);
 #pragma unroll
         for (int c = 0; c < kCols / 32; ++c) {
-          uint32_t r[32];
-          tmem_ld_32x32b_x32(taddr + c * 32, r);
-          tmem_wait_ld(r);
-          if (c + 1 == kCols / 32) release();
-          if constexpr (BVEC) {
-            const uint64_t a2 = pack_f32x2(cur_a, cur_a);
+          if (c + 1 < kCols / 32) tmem_ld_32x32b_x32(taddr + (c + 1) * 32, r[(c + 1) & 1]); else release();
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              uint64_t b0, b1;
-              ld_shared_2x64(sbuf + static_cast<uint32_t>(c * 32 + 4 * j) * 4u, b0, b1);
-              fma2_acc(acc[c * 16 + 2 * j], r[4 * j], r[4 * j + 1], mul2(a2, b0));
-              fma2_acc(acc[c * 16 + 2 * j + 1], r[4 * j + 2], r[4 * j + 3], mul2(a2, b1));
+          for (int j = 0; j < 16; j += 2) {
+            uint64_t c0 = s2, c1 = s2;
+            if constexpr (BVEC) {
+              ld_shared_2x64(cols + static_cast<uint32_t>(c * 32 + 2 * j) * 4u, c0, c1);
+              c0 = mul2(s2, c0);
+              c1 = mul2(s2, c1);
             }
-          } else {
-            const uint64_t s2 = pack_f32x2(s, s);
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              fma2_acc(acc[c * 16 + j], r[2 * j], r[2 * j + 1], s2);
+            fma2_acc(acc[c * 16 + j], r[c & 1][2 * j], r[c & 1][2 * j + 1], c0);
+            fma2_acc(acc[c * 16 + j + 1], r[c & 1][2 * j + 2], r[c & 1][2 * j + 3], c1);
           }
+          if (c + 1 < kCols / 32) tmem_wait_ld(r[(c + 1) & 1]);
         }
-      }
+        // Every lane has read its column scales (the row scale was read before release()).
+        if constexpr (BVEC) __syncwarp();
+        mbar_arrive_lane0(scale_empty + 8 * slot, lane);
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        if (++buf == kBufs) buf = 0;
+        if (++slot == S::kSlots) { slot = 0; slot_phase ^= 1; }
       }
       if (ok && active) block_output<kCols, OutT>(acc, n_first, row0, p, tma_c, stage_buf, lane);
     }
@@ -439,9 +488,10 @@ struct BlockConfig {
 
 BlockConfig select_block_config(int64_t m, int64_t n) {
   const int sms = current_sm_count();
-  const int64_t wide = ((m + 127) / 128) * ((n + 255) / 256);
-  if (const char* e = getenv("TB")) return BlockConfig{e[0] == 'p', atoi(e + 1)};
-  return wide >= sms ? BlockConfig{false, 256} : BlockConfig{false, 128};
+  // 256 x 256 tiles on CTA pairs where they fill the GPU at least half, else
+  // 128 x 128 tiles on single CTAs.
+  const int64_t pairs = ((m + 255) / 256) * ((n + 255) / 256);
+  return pairs * 4 >= sms ? BlockConfig{true, 256} : BlockConfig{false, 128};
 }
 
 template <typename Kern>
@@ -450,15 +500,11 @@ int launch_block(Kern kern, int smem, bool move_regs, std::atomic<uint64_t>& att
   if (int rc = set_smem_limit_once(kern, smem, attr_done, "cudaFuncSetAttribute(block-scaled GEMM)")) return rc;
   if (move_regs) {
     // The epilogue's larger share comes out of the launch's registers: it must be there.
-    static thread_local const void* checked = nullptr;
-    if (checked != reinterpret_cast<const void*>(kern)) {
-      cudaFuncAttributes fa{};
-      const cudaError_t e = cudaFuncGetAttributes(&fa, kern);
-      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncGetAttributes(block-scaled GEMM)");
-      if (fa.numRegs < 168)
-        return fail(CHOREO_ERR_UNSUPPORTED, "block-scaled GEMM: built with %d registers per thread, needs 168", fa.numRegs);
-      checked = reinterpret_cast<const void*>(kern);
-    }
+    cudaFuncAttributes fa{};
+    const cudaError_t e = cudaFuncGetAttributes(&fa, kern);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncGetAttributes(block-scaled GEMM)");
+    if (fa.numRegs < 168)
+      return fail(CHOREO_ERR_UNSUPPORTED, "block-scaled GEMM: built with %d registers per thread, needs 168", fa.numRegs);
   }
   const cudaError_t e = launch_pdl(kern, dim3(grid), dim3(kBlockThreads), smem, s, ta, tb, tc, kp);
   return e == cudaSuccess ? CHOREO_OK : cuda_fail(e, "block-scaled GEMM launch");
@@ -467,20 +513,10 @@ int launch_block(Kern kern, int smem, bool move_regs, std::atomic<uint64_t>& att
 template <bool BVEC, typename OutT>
 int dispatch_block(const BlockConfig& c, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc,
                    const BlockParams& kp, int grid, cudaStream_t s) {
-  if (c.pair && c.bn == 128) {
-    using S = BlockShape<true, 128>;
-    static std::atomic<uint64_t> done{0};
-    return launch_block(block_pair_kernel<128, BVEC, OutT>, S::kSmem, S::kMoveRegs, done, ta, tb, tc, kp, grid, s);
-  }
   if (c.pair) {
     using S = BlockShape<true, 256>;
     static std::atomic<uint64_t> done{0};
     return launch_block(block_pair_kernel<256, BVEC, OutT>, S::kSmem, S::kMoveRegs, done, ta, tb, tc, kp, grid, s);
-  }
-  if (c.bn == 256) {
-    using S = BlockShape<false, 256>;
-    static std::atomic<uint64_t> done{0};
-    return launch_block(block_single_kernel<256, BVEC, OutT>, S::kSmem, S::kMoveRegs, done, ta, tb, tc, kp, grid, s);
   }
   using S = BlockShape<false, 128>;
   static std::atomic<uint64_t> done{0};
@@ -623,7 +659,7 @@ int choreo_gemm_block_scaled_query(const choreo_gemm_block_desc* d, choreo_launc
   const BlockConfig c = select_block_config(d->m, d->n);
   out->tile_m = c.pair ? 256 : 128;
   out->tile_n = c.bn;
-  out->stages = BlockShape<true, 256>::kStages;
+  out->stages = c.pair ? BlockShape<true, 256>::kStages : BlockShape<false, 128>::kStages;
   out->cluster_m = c.pair ? 2 : 1;
   out->tiles = block_tiles(*d, c);
   out->grid_x = block_grid(out->tiles, c);
@@ -680,11 +716,11 @@ int choreo_gemm_block_scaled(const choreo_gemm_block_desc* d, void* stream) {
   if (kp.c_tma) {
     const uint64_t dims[3] = {static_cast<uint64_t>(d->n), static_cast<uint64_t>(d->m), 1};
     const uint64_t strides[2] = {static_cast<uint64_t>(d->ldc) * eb, static_cast<uint64_t>(d->m) * d->ldc * eb};
-    const uint32_t box[3] = {static_cast<uint32_t>(128 / eb), 32, 1};
+    const uint32_t box[3] = {static_cast<uint32_t>(64 / eb), 32, 1};
     const CUtensorMapDataType dt = d->dtype_c == CHOREO_DTYPE_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : d->dtype_c == CHOREO_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                                      : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    if ((rc = encode_tmap(&tc, dt, 3, d->c, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
+    if ((rc = encode_tmap(&tc, dt, 3, d->c, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B))) return rc;
   }
   kp.status = status_word();
   kp.timeout_ns = wait_timeout_ns();

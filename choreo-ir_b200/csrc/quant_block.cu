@@ -122,7 +122,11 @@ template <typename T>
 __device__ __forceinline__ void quantize_piece(const Piece<T>& v, float inv, bool clean, uint32_t (&q)[2]) {
   float f[Piece<T>::kElems];
 #pragma unroll
-  for (int i = 0; i < Piece<T>::kElems; ++i) f[i] = (clean ? v.get(i) : finite_or_nan(v.get(i))) * inv;
+  for (int i = 0; i < Piece<T>::kElems; ++i) f[i] = v.get(i) * inv;
+  if (!clean) {
+#pragma unroll
+    for (int i = 0; i < Piece<T>::kElems; ++i) f[i] = finite_or_nan(v.get(i)) * inv;
+  }
   q[0] = e4m3x4(f[0], f[1], f[2], f[3]);
   if constexpr (sizeof(T) == 2) q[1] = e4m3x4(f[4], f[5], f[6], f[7]);
 }
@@ -168,7 +172,8 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantParams p, in
     for (int o = kLanes / 2; o > 0; o >>= 1) top = top_max<T>(top, __shfl_xor_sync(0xffffffffu, top, o));
     bool clean;
     float amax = top_value<T>(top, &clean);
-    if (__any_sync(0xffffffffu, !clean)) {
+    clean = __all_sync(0xffffffffu, clean);
+    if (!clean) {
       float m = v[u].finite_top();
 #pragma unroll
       for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -325,7 +330,8 @@ __global__ void __launch_bounds__(256) quant_tile_kernel(const QuantParams p) {
 #pragma unroll
         for (int o = kLanes / 2; o > 0; o >>= 1) top = top_max<T>(top, __shfl_xor_sync(0xffffffffu, top, o));
         float amax = top_value<T>(top, &clean);
-        if (__any_sync(0xffffffffu, !clean)) {
+        clean = __all_sync(0xffffffffu, clean);
+        if (!clean) {
           float m = u.finite_top();
 #pragma unroll
           for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));

@@ -108,6 +108,39 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const W
   }
 }
 
+// Waits of a whole converged warp for one or two barriers: both are polled
+// before either result is looked at, and the branch on the outcome is the same
+// in every lane, so a wait that is over costs one round trip and leaves the
+// warp converged.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, const WaitCtx& w, uint32_t code) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, w, code));
+}
+__device__ __forceinline__ bool mbar_wait_warp2(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1,
+                                                const WaitCtx& w, uint32_t code) {
+  const bool a = mbar_try_wait(bar0, parity0);
+  const bool b = mbar_try_wait(bar1, parity1);
+  if (__all_sync(0xffffffffu, a && b)) return true;
+  return __all_sync(0xffffffffu, mbar_wait(bar0, parity0, w, code) && mbar_wait(bar1, parity1, w, code));
+}
+// Lane 0 arrives, without a branch (one would let its lanes run on apart).
+__device__ __forceinline__ void mbar_arrive_lane0(uint32_t bar, int lane) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.eq.s32 p, %1, 0;\n\t"
+      "@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(bar),
+      "r"(lane)
+      : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster_lane0(uint32_t cluster_addr, int lane) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.eq.s32 p, %1, 0;\n\t"
+      "@p mbarrier.arrive.shared::cluster.b64 _, [%0];\n\t}" ::"r"(cluster_addr),
+      "r"(lane)
+      : "memory");
+}
+
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
