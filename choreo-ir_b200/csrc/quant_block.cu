@@ -145,12 +145,41 @@ __device__ __forceinline__ void store_q(uint8_t* q, const uint32_t (&v)[2], int6
     if (i < left) q[i] = static_cast<uint8_t>(v[i / 4] >> (8 * (i & 3)));
 }
 
+// inv and scale of UNROLL blocks per lane group, from their amax: lane l of a
+// group divides for block l % UNROLL only and the group shares the factors (a
+// correctly rounded division is some 15 instructions, and as many as the rest
+// of a block's work if every lane did both for every block).
+template <int UNROLL>
+__device__ __forceinline__ float pick(const float (&v)[UNROLL], int i) {
+  float r = v[0];
+#pragma unroll
+  for (int u = 1; u < UNROLL; ++u) r = i == u ? v[u] : r;
+  return r;
+}
+
+// Largest finite magnitude of the kLanes lanes' pieces, in every lane of the
+// group; *clean: no NaN or infinity in the warp's pieces.
+template <typename T, int kLanes>
+__device__ __forceinline__ float group_amax(const Piece<T>& v, bool* clean) {
+  uint32_t top = v.top();
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) top = top_max<T>(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float amax = top_value<T>(top, clean);
+  *clean = __all_sync(0xffffffffu, *clean);
+  if (!*clean) {
+    amax = v.finite_top();
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  }
+  return amax;
+}
+
 // 1 x 128 blocks along X's rows. A block is 16 lanes' 16-byte loads (32 lanes'
 // for f32); a warp takes UNROLL consecutive 512-byte runs of one row, all loads
 // in flight at once, and 8 neighbouring rows share a CTA so that their scales
 // fall into one 32-byte sector. Bound by memory: 3 (5) bytes per element.
 template <typename T, int UNROLL>
-__global__ void __launch_bounds__(256) quant_rows_kernel(const QuantParams p, int64_t runs) {
+__global__ void __launch_bounds__(256, 5) quant_rows_kernel(const QuantParams p, int64_t runs) {
   constexpr int E = Piece<T>::kElems;
   constexpr int kLanes = 128 / E;  // lanes of one block
   griddep_wait();
@@ -159,35 +188,32 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantParams p, in
   const int64_t group = blockIdx.x / runs;
   const int64_t r = group * 8 + warp;
   if (r >= p.rows) return;
-  const int64_t c0 = (blockIdx.x - group * runs) * (UNROLL * 32 * E) + lane * E;
+  const int64_t run0 = (blockIdx.x - group * runs) * (UNROLL * 32 * E);
+  const int64_t c0 = run0 + lane * E;
   const T* x = static_cast<const T*>(p.x) + r * p.ldx + c0;
   Piece<T> v[UNROLL];
 #pragma unroll
   for (int u = 0; u < UNROLL; ++u) v[u].load(x + u * 32 * E, p.cols - c0 - u * 32 * E);
+  float amax[UNROLL];
+  bool clean[UNROLL];
+#pragma unroll
+  for (int u = 0; u < UNROLL; ++u) amax[u] = group_amax<T, kLanes>(v[u], &clean[u]);
+  const int mine = lane % kLanes;
+  const float own = pick<UNROLL>(amax, mine % UNROLL);
+  const float inv = factor_of(own);
+  const int64_t own_col = run0 + mine * 32 * E + lane / kLanes * 128;
+  if (mine < UNROLL && own_col < p.cols) p.scale[r * p.scale_row + own_col / 128 * p.scale_blk] = scale_of(own);
 #pragma unroll
   for (int u = 0; u < UNROLL; ++u) {
     const int64_t c = c0 + u * 32 * E;
-    uint32_t top = v[u].top();
-#pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) top = top_max<T>(top, __shfl_xor_sync(0xffffffffu, top, o));
-    bool clean;
-    float amax = top_value<T>(top, &clean);
-    clean = __all_sync(0xffffffffu, clean);
-    if (!clean) {
-      float m = v[u].finite_top();
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      amax = m;
-    }
     uint32_t q[2];
-    quantize_piece<T>(v[u], factor_of(amax), clean, q);
+    quantize_piece<T>(v[u], __shfl_sync(0xffffffffu, inv, (lane & ~(kLanes - 1)) | u), clean[u], q);
     store_q<E>(p.q + r * p.ldq + c, q, p.cols - c, p.q_vec != 0);
-    if (lane % kLanes == 0 && c < p.cols) p.scale[r * p.scale_row + c / 128 * p.scale_blk] = scale_of(amax);
   }
 }
 
-// Largest finite magnitude over the CTA's 256 threads.
-template <typename T>
+// Largest finite magnitude over the CTA's threads.
+template <typename T, int kWarps>
 __device__ __forceinline__ float cta_amax(uint32_t top, float finite_top, uint32_t* warp_top, float* warp_finite,
                                           bool* all_clean) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -204,7 +230,7 @@ __device__ __forceinline__ float cta_amax(uint32_t top, float finite_top, uint32
   float m = 0.f;
   bool all = true;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) {
+  for (int w = 0; w < kWarps; ++w) {
     bool clean;
     top_value<T>(warp_top[w], &clean);
     all = all && clean;
@@ -222,16 +248,17 @@ __device__ __forceinline__ float cta_amax(uint32_t top, float finite_top, uint32
 // X, 4 for f32), chunk j of row c stored at j ^ (c / elements per load): a
 // warp's store touches 4 words of a chunk in 8 different chunks, its load of
 // whole chunks 8 different chunks per 8 lanes, both without bank conflicts.
-template <typename T, bool SQUARE, bool TRANS>
-__global__ void __launch_bounds__(256) quant_tile_kernel(const QuantParams p) {
+template <typename T, bool SQUARE, bool TRANS, int kThreads>
+__global__ void __launch_bounds__(kThreads) quant_tile_kernel(const QuantParams p) {
+  constexpr int kWarps = kThreads / 32;
   constexpr int E = Piece<T>::kElems;        // elements of a load; rows of X in a chunk
-  constexpr int kPieces = 128 * 128 / E / 256;
+  constexpr int kPieces = 128 * 128 / E / kThreads;
   constexpr int kLanes = 128 / E;
   constexpr int kWords = 128 * static_cast<int>(sizeof(T)) / 4;  // 32-bit words of a tile row
   extern __shared__ uint4 turned_raw[];
   uint32_t* turned = reinterpret_cast<uint32_t*>(turned_raw);
-  __shared__ uint32_t warp_top[8];
-  __shared__ float warp_finite[8];
+  __shared__ uint32_t warp_top[kWarps];
+  __shared__ float warp_finite[kWarps];
   griddep_wait();
   griddep_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -244,7 +271,7 @@ __global__ void __launch_bounds__(256) quant_tile_kernel(const QuantParams p) {
     constexpr int kRows = 32 / kLanes;  // rows of one warp load
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
-      const int64_t r = r0 + (i * 8 + warp) * kRows + lane / kLanes;
+      const int64_t r = r0 + (i * kWarps + warp) * kRows + lane / kLanes;
       const int64_t c = c0 + lane % kLanes * E;
       v[i].load(x + (r < p.rows ? r : p.rows - 1) * p.ldx + c, r < p.rows ? p.cols - c : 0);
     }
@@ -255,7 +282,7 @@ __global__ void __launch_bounds__(256) quant_tile_kernel(const QuantParams p) {
     constexpr int kPair = 4 / static_cast<int>(sizeof(T)) ;  // rows of X in one word
 #pragma unroll
     for (int i = 0; i < kPieces / kPair; ++i) {
-      const int unit = i * 8 + warp;         // (chunk, group)
+      const int unit = i * kWarps + warp;    // (chunk, group)
       const int chunk = unit / kGroups, grp = unit % kGroups;
 #pragma unroll
       for (int h = 0; h < kPair; ++h) {
@@ -281,7 +308,7 @@ __global__ void __launch_bounds__(256) quant_tile_kernel(const QuantParams p) {
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) m = fmaxf(m, v[i].finite_top());
     }
-    const float amax = cta_amax<T>(top, m, warp_top, warp_finite, &clean);
+    const float amax = cta_amax<T, kWarps>(top, m, warp_top, warp_finite, &clean);
     inv = factor_of(amax);
     if (threadIdx.x == 0) p.scale[rt * p.scale_row + ct * p.scale_blk] = scale_of(amax);
   }
@@ -290,7 +317,7 @@ __global__ void __launch_bounds__(256) quant_tile_kernel(const QuantParams p) {
     constexpr int kRows = 32 / kLanes;
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
-      const int64_t r = r0 + (i * 8 + warp) * kRows + lane / kLanes;
+      const int64_t r = r0 + (i * kWarps + warp) * kRows + lane / kLanes;
       const int64_t c = c0 + lane % kLanes * E;
       if (r >= p.rows) continue;
       uint32_t q[2];
@@ -302,7 +329,7 @@ __global__ void __launch_bounds__(256) quant_tile_kernel(const QuantParams p) {
     constexpr int kPair = 4 / static_cast<int>(sizeof(T));
 #pragma unroll
     for (int i = 0; i < kPieces / kPair; ++i) {
-      const int unit = i * 8 + warp;
+      const int unit = i * kWarps + warp;
       const int chunk = unit / kGroups, grp = unit % kGroups;
       const int piece = grp * 8 + (lane & 7);  // columns of X piece * E .. + E - 1
       uint32_t* dst = turned + piece * E * kWords + ((chunk ^ piece) * 4 + (lane >> 3));
@@ -318,33 +345,37 @@ __global__ void __launch_bounds__(256) quant_tile_kernel(const QuantParams p) {
     }
     __syncthreads();
     constexpr int kRows = 32 / kLanes;  // rows of op(X) of one warp load
+    constexpr int kSteps = 128 / kWarps / kRows;
+    constexpr int kStep = kSteps < 4 ? kSteps : 4;  // rows in registers at once
     const int part = lane % kLanes;
-#pragma unroll 4
-    for (int i = 0; i < 128 / 8 / kRows; ++i) {
-      const int row = (i * 8 + warp) * kRows + lane / kLanes;
-      Piece<T> u;
-      const uint4 w = *reinterpret_cast<const uint4*>(turned + row * kWords + (part ^ (row / E)) * 4);
-      u.w[0] = w.x, u.w[1] = w.y, u.w[2] = w.z, u.w[3] = w.w;
-      if constexpr (!SQUARE) {
-        uint32_t top = u.top();
+    const int64_t c = c0 + part * E;
+#pragma unroll 1
+    for (int i0 = 0; i0 < kSteps; i0 += kStep) {
+      auto row_of = [&](int i) { return ((i0 + i) * kWarps + warp) * kRows + lane / kLanes; };
+      Piece<T> u[kStep];
+      float amax[kStep];
+      bool ok[kStep];
 #pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) top = top_max<T>(top, __shfl_xor_sync(0xffffffffu, top, o));
-        float amax = top_value<T>(top, &clean);
-        clean = __all_sync(0xffffffffu, clean);
-        if (!clean) {
-          float m = u.finite_top();
-#pragma unroll
-          for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-          amax = m;
-        }
-        inv = factor_of(amax);
-        if (part == 0 && r0 + row < p.rows) p.scale[(r0 + row) * p.scale_row + ct * p.scale_blk] = scale_of(amax);
+      for (int i = 0; i < kStep; ++i) {
+        const int row = row_of(i);
+        const uint4 w = *reinterpret_cast<const uint4*>(turned + row * kWords + (part ^ (row / E)) * 4);
+        u[i].w[0] = w.x, u[i].w[1] = w.y, u[i].w[2] = w.z, u[i].w[3] = w.w;
+        ok[i] = clean;
+        if constexpr (!SQUARE) amax[i] = group_amax<T, kLanes>(u[i], &ok[i]);
       }
-      const int64_t c = c0 + part * E;
-      if (r0 + row < p.rows) {
+      if constexpr (!SQUARE) {
+        const float own = pick<kStep>(amax, part % kStep);
+        inv = factor_of(own);
+        const int64_t r = r0 + row_of(part);
+        if (part < kStep && r < p.rows) p.scale[r * p.scale_row + ct * p.scale_blk] = scale_of(own);
+      }
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) {
+        const int64_t r = r0 + row_of(i);
+        const float f = SQUARE ? inv : __shfl_sync(0xffffffffu, inv, (lane & ~(kLanes - 1)) | i);
         uint32_t q[2];
-        quantize_piece<T>(u, inv, clean, q);
-        store_q<E>(p.q + (r0 + row) * p.ldq + c, q, p.cols - c, p.q_vec != 0);
+        quantize_piece<T>(u[i], f, ok[i], q);
+        if (r < p.rows) store_q<E>(p.q + r * p.ldq + c, q, p.cols - c, p.q_vec != 0);
       }
     }
   }
@@ -385,7 +416,7 @@ __global__ void __launch_bounds__(256) quant_unaligned_kernel(const QuantParams 
 #pragma unroll
       for (int j = 0; j < 4; ++j) m = fmaxf(m, finite_abs(tile[i * 129 + lane + 32 * j]));
     bool clean;
-    const float amax = cta_amax<float>(0, m, warp_top, warp_finite, &clean);
+    const float amax = cta_amax<float, 8>(0, m, warp_top, warp_finite, &clean);
     inv = factor_of(amax);
     if (threadIdx.x == 0) p.scale[rt * p.scale_row + ct * p.scale_blk] = scale_of(amax);
   }
@@ -417,11 +448,12 @@ using namespace choreo_sm100;
 namespace {
 
 template <typename Kern, typename... Args>
-int launch_quant(Kern kern, int64_t grid, int smem, std::atomic<uint64_t>& done, cudaStream_t s, Args... args) {
+int launch_quant(Kern kern, int64_t grid, int threads, int smem, std::atomic<uint64_t>& done, cudaStream_t s,
+                 Args... args) {
   if (grid > INT32_MAX) return fail(CHOREO_ERR_UNSUPPORTED, "quantize: more than 2^31-1 tiles");
   if (smem > 0)
     if (int rc = set_smem_limit_once(kern, smem, done, "cudaFuncSetAttribute(quantize)")) return rc;
-  const cudaError_t e = launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(256), smem, s, args...);
+  const cudaError_t e = launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(threads), smem, s, args...);
   return e == cudaSuccess ? CHOREO_OK : cuda_fail(e, "quantize launch");
 }
 
@@ -430,7 +462,7 @@ int launch_rows(const QuantParams& p, cudaStream_t s) {
   constexpr int64_t span = UNROLL * 32 * Piece<T>::kElems;
   const int64_t runs = (p.cols + span - 1) / span;
   std::atomic<uint64_t> none{0};
-  return launch_quant(quant_rows_kernel<T, UNROLL>, (p.rows + 7) / 8 * runs, 0, none, s, p, runs);
+  return launch_quant(quant_rows_kernel<T, UNROLL>, (p.rows + 7) / 8 * runs, 256, 0, none, s, p, runs);
 }
 
 template <typename T, bool SQUARE, bool TRANS>
@@ -438,12 +470,13 @@ int launch_tile(const QuantParams& p, bool x_vec, cudaStream_t s) {
   const int64_t grid = p.row_tiles * p.col_tiles;
   if (!x_vec) {
     static std::atomic<uint64_t> done{0};
-    return launch_quant(quant_unaligned_kernel<T, SQUARE, TRANS>, grid, 128 * 129 * 4, done, s, p);
+    return launch_quant(quant_unaligned_kernel<T, SQUARE, TRANS>, grid, 256, 128 * 129 * 4, done, s, p);
   }
   if constexpr (SQUARE || TRANS) {
     static std::atomic<uint64_t> done{0};
-    return launch_quant(quant_tile_kernel<T, SQUARE, TRANS>, grid, TRANS ? 128 * 128 * static_cast<int>(sizeof(T)) : 0,
-                        done, s, p);
+    constexpr int kThreads = 256;
+    return launch_quant(quant_tile_kernel<T, SQUARE, TRANS, kThreads>, grid, kThreads,
+                        TRANS ? 128 * 128 * static_cast<int>(sizeof(T)) : 0, done, s, p);
   } else {
     // Four loads in flight a thread where that still leaves every SM two CTAs;
     // a few rows are spread over as many SMs as one load each can reach.

@@ -18,9 +18,11 @@
 #include <type_traits>
 
 #include "compute/auto_analyze.hpp"
+#include "compute/block_scaled.hpp"
 #include "compute/compute.hpp"
 #include "compute/conv.hpp"
 #include "compute/elementwise.hpp"
+#include "compute/gated_ffn.hpp"
 #include "compute/host_pipeline.hpp"
 #include "compute/matmul.hpp"
 #include "compute/validation.hpp"
