@@ -469,13 +469,17 @@ def _act_code(act):
     return _ACTS[act]
 
 
-def _workspace(need, workspace, device):
-    """(tensor, bytes): the caller's workspace, or one of `need` bytes."""
+def _workspace(need, workspace, device, stream):
+    """(tensor, bytes): the caller's workspace, or one of `need` bytes. Memory
+    allocated here belongs to torch's current stream: where the call runs on
+    another one, it is not handed out again before that one has passed the call."""
     if workspace is None:
         if not need:
             return None, 0
         import torch
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        if stream is not None:
+            workspace.record_stream(torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream)
     return workspace, workspace.numel() * workspace.element_size()
 
 
@@ -514,15 +518,15 @@ def gated_ffn(x, w_gate, w_up, h, *, act="silu", trans_w=False, gate=None, up=No
     and up, when given, receive the two products for gated_ffn_backward. Rows
     may be padded. All are f16, or all bf16."""
     d = ffn_desc(x, w_gate, w_up, h, act=act, trans_w=trans_w, gate=gate, up=up)
-    stream = _stream_ptr(stream)
+    ptr = _stream_ptr(stream)
     if workspace is None:
         # aligned operands need none: ask for the size only when the call does
-        rc = lib.choreo_gated_ffn(C.byref(d), None, 0, stream)
+        rc = lib.choreo_gated_ffn(C.byref(d), None, 0, ptr)
         if rc != ERR_WORKSPACE:
             return check(rc)
     need = gated_ffn_query(d).workspace_bytes if workspace is None else 0
-    workspace, ws_bytes = _workspace(need, workspace, h.device)
-    check(lib.choreo_gated_ffn(C.byref(d), _ptr(workspace), ws_bytes, stream))
+    workspace, ws_bytes = _workspace(need, workspace, h.device, stream)
+    check(lib.choreo_gated_ffn(C.byref(d), _ptr(workspace), ws_bytes, ptr))
 
 
 def ffn_grad_desc(dh, x, w_gate, w_up, *, dx=None, dw_gate=None, dw_up=None, gate=None, up=None, h=None, act="silu",
@@ -555,7 +559,7 @@ def gated_ffn_backward(dh, x, w_gate, w_up, *, dx=None, dw_gate=None, dw_up=None
     d = ffn_grad_desc(dh, x, w_gate, w_up, dx=dx, dw_gate=dw_gate, dw_up=dw_up, gate=gate, up=up, h=h, act=act,
                       trans_w=trans_w, accumulate=accumulate)
     need = gated_ffn_backward_query(d).workspace_bytes if workspace is None else 0
-    workspace, ws_bytes = _workspace(need, workspace, dh.device)
+    workspace, ws_bytes = _workspace(need, workspace, dh.device, stream)
     check(lib.choreo_gated_ffn_backward(C.byref(d), _ptr(workspace), ws_bytes, _stream_ptr(stream)))
 
 

@@ -7,6 +7,13 @@
 // accumulator in TMEM. The epilogue warps read it out, multiply by the two
 // scales and add it to the tile's fp32 sum, which stays in their registers for
 // the whole tile; the next block runs meanwhile in the other accumulator.
+//
+// Bound by the fp32 sums of the epilogue, not by the MMAs: a 256 x 256 tile's
+// k-block takes 512 cycles of MMAs and 848 in all (1342 with a scale per column,
+// which doubles the arithmetic: a product of the two scales and the sum for
+// every element). Long calls are bound by the 1 kW cap before that: 8192^3 bf16
+// out 604-639 us = 1.7-1.8 PFLOP/s at 1.2 GHz, 4096^3 91 us, the f32 weight
+// gradient 4096 x 10240 x 8192 with both scales per row 566 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -20,6 +20,11 @@
 // act(G) * U. kBlock: e4m3 weights and tokens with scales; as in the large
 // tiles every k-block is one scale block with an accumulator of its own, added
 // to fp32 sums in registers.
+//
+// Measured: 1 x 4096 x 10240 bf16 gate, weights N x K, 29.6 us = 0.86 of the
+// copy bandwidth (K x N: 25.9 us = 0.99); 16 x 10240 x 4096 in 8 bits 13.1 us
+// for 6.5 us of bytes, the rest the start of ten k-blocks a CTA and the
+// reduction over 8 CTAs.
 #pragma once
 #include <algorithm>
 

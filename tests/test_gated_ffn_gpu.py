@@ -375,6 +375,27 @@ def test_repeats_bit_for_bit_on_streams_and_in_graphs(cb, cuda):
             assert torch.equal(o[name], ref[name]), name
 
 
+def test_workspace_outlives_a_call_on_another_stream(cb, cuda):
+    """The binding's own workspace (dG and dU, and repacked operands) is not
+    handed to the current stream's allocations while a call on an explicit
+    stream still uses it."""
+    import torch
+    c = Case(500, 1003, 331, "bf16", "silu", False, pads=(1, 1, 0))   # unaligned: repacks as well
+    ref = torch.empty(500, 331, device="cuda", dtype=c.dt)
+    cb.gated_ffn_backward(c.dh, c.x, c.wg, c.wu, dx=ref)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    for stream in (s, s.cuda_stream):
+        outs = [torch.empty_like(ref) for _ in range(8)]
+        torch.cuda.synchronize()
+        for o in outs:
+            cb.gated_ffn_backward(c.dh, c.x, c.wg, c.wu, dx=o, stream=stream)
+            torch.empty(4 * 500 * 1008 * 2, dtype=torch.uint8, device="cuda").fill_(0x7F)  # current stream
+        torch.cuda.synchronize()
+        for o in outs:
+            assert torch.equal(o, ref)
+
+
 def test_feed_forward_block_with_an_8_bit_down_projection(cb, cuda):
     """x -> gated_ffn -> quantize_block -> gemm_block_scaled with the residual
     as addend, for a prompt and for one token, against the 64-bit block. The
