@@ -41,8 +41,9 @@ struct BlockParams : TcParams {
 
 template <int STAGES, int BUFS>
 struct alignas(8) BlockBarriers {
+  uint64_t half[STAGES];      // tiles in halves: the first half's MMAs are done, its accumulator is full
   uint64_t full[STAGES];      // the stage's tiles have landed
-  uint64_t empty[STAGES];     // its MMAs are done: the stage is free, its block's accumulator is full
+  uint64_t empty[STAGES];     // all its MMAs are done: the stage is free, the (other half's) accumulator is full
   uint64_t tmem_empty[BUFS];  // the epilogue has read the accumulator
   uint64_t scale_full[4];     // a block's scales are in their slot
   uint64_t scale_empty[4];    // the epilogue has read them
@@ -59,7 +60,10 @@ struct BlockShape {
   static constexpr uint32_t kBStage = kBRows * kBlockK;
   static constexpr int kStages = 6;
   static constexpr int kBufs = 512 / BN;  // block accumulators in TMEM
-  using Barriers = BlockBarriers<kStages, kBufs>;
+  // 256-column tiles are two MMAs of 128 columns with an accumulator each: half
+  // h is 64 columns of each CTA's B rows, tile columns 64 h .. and 128 + 64 h ..
+  static constexpr int kHalves = PAIR && BN == 256 ? 2 : 1;
+  using Barriers = BlockBarriers<kStages, kBufs * kHalves>;
   static constexpr uint32_t kStaging = kEpiWarps * 2048;             // 32 rows x 64 bytes a warp
   static constexpr int kSlots = 4;                                   // scale slots
   static constexpr uint32_t kSlotFloats = 128 + (BN > 128 ? BN : 128);  // rows', then columns' (see the scale warps)
@@ -103,7 +107,7 @@ __device__ __forceinline__ void ld_shared_2x64(uint32_t addr, uint64_t& a, uint6
 // 16-byte chunk j of row r at j ^ (r / 2 % 4)) and bulk tensor stores, or
 // element by element where those are not legal.
 template <int kCols, typename OutT>
-__device__ __forceinline__ void block_output(const uint64_t (&acc)[kCols / 2], int n_first, int row0, const BlockParams& p,
+__device__ __forceinline__ void block_output(const uint64_t (&acc)[kCols / 2], int n_first, int n_second, int row0, const BlockParams& p,
                                              const CUtensorMap* tma_c, uint32_t stage_buf, int lane) {
   constexpr int E = 64 / static_cast<int>(sizeof(OutT));  // columns per staging row
   const int row = row0 + lane;
@@ -116,8 +120,9 @@ __device__ __forceinline__ void block_output(const uint64_t (&acc)[kCols / 2], i
   const int sw = (lane >> 1) & 3;
 #pragma unroll
   for (int c = 0; c < kCols / 32; ++c) {
-    const int n_base = n_first + c * 32;
-    if (n_base >= p.n) break;  // warp-uniform
+    // the warp's first 64 columns start at n_first, the others at n_second
+    const int n_base = c < 2 ? n_first + c * 32 : n_second + (c - 2) * 32;
+    if (n_base >= p.n) continue;  // warp-uniform
     uint32_t r[32];
 #pragma unroll
     for (int i = 0; i < 16; ++i)
@@ -168,6 +173,8 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
   constexpr int kCols = BN / 2;  // columns of one epilogue warp
   constexpr uint32_t kTmemCols = 512;
   constexpr int kBufs = S::kBufs;
+  constexpr int kHalves = S::kHalves;
+  constexpr int kHalfN = BN / kHalves;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
@@ -188,9 +195,10 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(smem_u32(&bars->full[s]), 1);
       mbar_init(smem_u32(&bars->empty[s]), 1);
+      mbar_init(smem_u32(&bars->half[s]), 1);
     }
-    for (int i = 0; i < kBufs; ++i) {
-      mbar_init(smem_u32(&bars->tmem_empty[i]), (PAIR ? 2 : 1) * kEpiWarps);
+    for (int i = 0; i < kBufs * kHalves; ++i) {
+      mbar_init(smem_u32(&bars->tmem_empty[i]), (PAIR ? 2 : 1) * kEpiWarps / kHalves);
     }
     for (int i = 0; i < S::kSlots; ++i) {
       mbar_init(smem_u32(&bars->scale_full[i]), 2);
@@ -271,30 +279,44 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
       // so it holds little: descriptors and barrier addresses
       // advance by additions, and one commit per k-block tells the producer
       // that the stage is free and the epilogue that its accumulator is full.
-      constexpr uint32_t idesc = idesc_e4m3(kTileM, BN);
+      constexpr uint32_t idesc = idesc_e4m3(kTileM, kHalfN);
       const uint64_t desc_a = smem_desc_sw128(smem_u32(s_a), 16, 1024);
       const uint64_t desc_b = smem_desc_sw128(smem_u32(s_b), 16, 1024);
       const uint32_t bar_full = smem_u32(&bars->full[0]), bar_done = smem_u32(&bars->empty[0]);
+      const uint32_t bar_half = smem_u32(&bars->half[0]);
       const uint32_t bar_free = smem_u32(&bars->tmem_empty[0]);
       uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 1;
       const int64_t blocks = (p.num_tiles - first + step - 1) / step * p.num_k_blocks;
       for (int64_t i = 0; i < blocks; ++i) {
-        if (!mbar_wait_warp2(bar_full + 8 * stage, phase, bar_free + 8 * buf, buf_phase, wctx, kStatusTimeoutMma)) break;
+        if (!mbar_wait_warp2(bar_full + 8 * stage, phase, bar_free + 8 * kHalves * buf, buf_phase, wctx,
+                             kStatusTimeoutMma))
+          break;
         tc_fence_after();
         const uint64_t ad = smem_desc_advance(desc_a, stage * S::kAStage);
-        const uint64_t bd = smem_desc_advance(desc_b, stage * S::kBStage);
-        const uint32_t d = tmem_base + buf * BN;
-        if (elect_one()) {
+        bool ok = true;
 #pragma unroll
-          for (uint32_t k = 0; k < kBlockK / 32; ++k) {
-            if constexpr (PAIR)
-              umma_f8_pair(d, smem_desc_advance(ad, k * 32), smem_desc_advance(bd, k * 32), idesc, k != 0 ? 1u : 0u);
-            else
-              umma_f8(d, smem_desc_advance(ad, k * 32), smem_desc_advance(bd, k * 32), idesc, k != 0 ? 1u : 0u);
+        for (uint32_t h = 0; h < kHalves; ++h) {
+          if (h > 0) {
+            ok = mbar_wait_warp(bar_free + 8 * (kHalves * buf + h), buf_phase, wctx, kStatusTimeoutMma);
+            if (!ok) break;
+            tc_fence_after();
           }
-          if constexpr (PAIR) umma_commit_pair_both(bar_done + 8 * stage); else umma_commit(bar_done + 8 * stage);
+          const uint64_t bd = smem_desc_advance(desc_b, stage * S::kBStage + h * (S::kBStage / kHalves));
+          const uint32_t d = tmem_base + buf * BN + h * kHalfN;
+          if (elect_one()) {
+#pragma unroll
+            for (uint32_t k = 0; k < kBlockK / 32; ++k) {
+              if constexpr (PAIR)
+                umma_f8_pair(d, smem_desc_advance(ad, k * 32), smem_desc_advance(bd, k * 32), idesc, k != 0 ? 1u : 0u);
+              else
+                umma_f8(d, smem_desc_advance(ad, k * 32), smem_desc_advance(bd, k * 32), idesc, k != 0 ? 1u : 0u);
+            }
+            const uint32_t done = (h + 1 == kHalves ? bar_done : bar_half) + 8 * stage;
+            if constexpr (PAIR) umma_commit_pair_both(done); else umma_commit(done);
+          }
+          __syncwarp();
         }
-        __syncwarp();
+        if (!ok) break;
         if (++stage == STAGES) { stage = 0; phase ^= 1; }
         if (++buf == kBufs) { buf = 0; buf_phase ^= 1; }
       }
@@ -384,12 +406,18 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
     const int col_half = (warp - 4) >> 2;
     const uint32_t stage_buf = smem_u32(s_stage) + static_cast<uint32_t>(warp - 4) * 2048u;
     const uint32_t tmem_warp = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + col_half * kCols;
-    const uint32_t bar_done = smem_u32(&bars->empty[0]);
-    const uint32_t bar_free = PAIR ? mapa_shared(smem_u32(&bars->tmem_empty[0]), 0) : smem_u32(&bars->tmem_empty[0]);
+    // its accumulator: half col_half of the tile (halves), or the tile's
+    const int half = kHalves == 2 ? col_half : 0;
+    const uint32_t bar_done = smem_u32(kHalves == 2 && half == 0 ? &bars->half[0] : &bars->empty[0]);
+    const uint32_t own_free = smem_u32(&bars->tmem_empty[half]);
+    const uint32_t bar_free = PAIR ? mapa_shared(own_free, 0) : own_free;
+    // first columns of its first and second 64 within the tile
+    const int seg0 = kHalves == 2 ? 64 * half : col_half * kCols;
+    const int seg1 = kHalves == 2 ? 128 + 64 * half : seg0 + 64;
     const uint32_t scale_full = smem_u32(&bars->scale_full[0]), scale_empty = smem_u32(&bars->scale_empty[0]);
     // this lane's row scale, and the warp's column scales, in slot 0
-    const uint32_t scale_row = smem_u32(s_scale) + static_cast<uint32_t>((BVEC ? 0 : col_half * 128) + quarter * 32 + lane) * 4u;
-    const uint32_t scale_col = smem_u32(s_scale) + static_cast<uint32_t>(128 + col_half * kCols) * 4u;
+    const uint32_t scale_row = smem_u32(s_scale) + static_cast<uint32_t>((BVEC || kHalves == 2 ? 0 : col_half * 128) + quarter * 32 + lane) * 4u;
+    const uint32_t scale_col = smem_u32(s_scale) + 128u * 4u;
     griddep_wait();
     uint32_t stage = 0, phase = 0, buf = 0, slot = 0, slot_phase = 0;
     bool ok = true;
@@ -397,7 +425,7 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
       int b, mb, nb;
       tile_coords(t, p, b, mb, nb);
       const int row0 = mb * kTileM + static_cast<int>(rank) * kBM + quarter * 32;
-      const int n_first = nb * BN + col_half * kCols;
+      const int n_first = nb * BN + seg0;
       const bool active = row0 < p.m && n_first < p.n;
       uint64_t acc[kCols / 2];  // the warp's sums, in pairs of columns
 #pragma unroll
@@ -421,13 +449,19 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
         const float s = ld_shared_f32(scale_row + slot * (S::kSlotFloats * 4));
         const uint32_t cols = scale_col + slot * (S::kSlotFloats * 4);
         const uint64_t s2 = pack_f32x2(s, s);
+        // halves: the second 64 columns lie in B's next 128 rows
+        uint64_t s2_second = s2;
+        if constexpr (kHalves == 2 && !BVEC) {
+          const float second = ld_shared_f32(scale_row + slot * (S::kSlotFloats * 4) + 512u);
+          s2_second = pack_f32x2(second, second);
+        }
         auto release = [&] {
           tc_fence_before();
           __syncwarp();
           if constexpr (PAIR)
-            mbar_arrive_cluster_lane0(bar_free + 8 * buf, lane);
+            mbar_arrive_cluster_lane0(bar_free + 8 * kHalves * buf, lane);
           else
-            mbar_arrive_lane0(bar_free + 8 * buf, lane);
+            mbar_arrive_lane0(bar_free + 8 * kHalves * buf, lane);
         };
         tmem_wait_ld(r[0]);
 #pragma unroll
@@ -435,9 +469,9 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
           if (c + 1 < kCols / 32) tmem_ld_32x32b_x32(taddr + (c + 1) * 32, r[(c + 1) & 1]); else release();
 #pragma unroll
           for (int j = 0; j < 16; j += 2) {
-            uint64_t c0 = s2, c1 = s2;
+            uint64_t c0 = c < 2 ? s2 : s2_second, c1 = c0;
             if constexpr (BVEC) {
-              ld_shared_2x64(cols + static_cast<uint32_t>(c * 32 + 2 * j) * 4u, c0, c1);
+              ld_shared_2x64(cols + static_cast<uint32_t>((c < 2 ? seg0 + c * 32 : seg1 + (c - 2) * 32) + 2 * j) * 4u, c0, c1);
               c0 = mul2(s2, c0);
               c1 = mul2(s2, c1);
             }
@@ -453,7 +487,7 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
         if (++buf == kBufs) buf = 0;
         if (++slot == S::kSlots) { slot = 0; slot_phase ^= 1; }
       }
-      if (ok && active) block_output<kCols, OutT>(acc, n_first, row0, p, tma_c, stage_buf, lane);
+      if (ok && active) block_output<kCols, OutT>(acc, n_first, nb * BN + seg1, row0, p, tma_c, stage_buf, lane);
     }
     if (lane == 0) bulk_wait_read_all();
     __syncwarp();
