@@ -9,11 +9,11 @@
 // the whole tile; the next block runs meanwhile in the other accumulator.
 //
 // Bound by the fp32 sums of the epilogue, not by the MMAs: a 256 x 256 tile's
-// k-block takes 512 cycles of MMAs and 848 in all (1342 with a scale per column,
+// k-block takes 512 cycles of MMAs and 729 in all (1334 with a scale per column,
 // which doubles the arithmetic: a product of the two scales and the sum for
-// every element). Long calls are bound by the 1 kW cap before that: 8192^3 bf16
-// out 604-639 us = 1.7-1.8 PFLOP/s at 1.2 GHz, 4096^3 91 us, the f32 weight
-// gradient 4096 x 10240 x 8192 with both scales per row 566 us.
+// every element), and on long calls by the 1 kW cap: 8192^3 with bf16 output
+// 539 us = 2.04 PFLOP/s, 4096^3 80 us, the f32 weight gradient 4096 x 10240 x
+// 8192 with both scales per row 570 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -26,7 +26,7 @@
 
 namespace choreo_sm100 {
 
-constexpr int kBlockThreads = 384;  // warpgroup 0: producer, MMA issuer; warpgroups 1 and 2: epilogue
+constexpr int kBlockThreads = 384;  // warpgroup 0: producer, MMA issuer, scales; warpgroups 1 and 2: epilogue
 constexpr int kBlockK = 128;        // e4m3 elements (bytes) per k-block
 
 struct BlockParams : TcParams {
@@ -62,6 +62,9 @@ struct BlockShape {
   static constexpr int kBufs = 512 / BN;  // block accumulators in TMEM
   // 256-column tiles are two MMAs of 128 columns with an accumulator each: half
   // h is 64 columns of each CTA's B rows, tile columns 64 h .. and 128 + 64 h ..
+  // The two epilogue warps of an SM sub-partition take one half each, so they
+  // work half a k-block apart, one's waits under the other's arithmetic (848 ->
+  // 729 cycles a k-block, 8192^3 638 -> 539 us).
   static constexpr int kHalves = PAIR && BN == 256 ? 2 : 1;
   using Barriers = BlockBarriers<kStages, kBufs * kHalves>;
   static constexpr uint32_t kStaging = kEpiWarps * 2048;             // 32 rows x 64 bytes a warp
@@ -107,8 +110,9 @@ __device__ __forceinline__ void ld_shared_2x64(uint32_t addr, uint64_t& a, uint6
 // 16-byte chunk j of row r at j ^ (r / 2 % 4)) and bulk tensor stores, or
 // element by element where those are not legal.
 template <int kCols, typename OutT>
-__device__ __forceinline__ void block_output(const uint64_t (&acc)[kCols / 2], int n_first, int n_second, int row0, const BlockParams& p,
-                                             const CUtensorMap* tma_c, uint32_t stage_buf, int lane) {
+__device__ __forceinline__ void block_output(const uint64_t (&acc)[kCols / 2], int n_first, int n_second, int row0,
+                                             const BlockParams& p, const CUtensorMap* tma_c, uint32_t stage_buf,
+                                             int lane) {
   constexpr int E = 64 / static_cast<int>(sizeof(OutT));  // columns per staging row
   const int row = row0 + lane;
   const bool row_ok = row < p.m;
@@ -197,9 +201,8 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
       mbar_init(smem_u32(&bars->empty[s]), 1);
       mbar_init(smem_u32(&bars->half[s]), 1);
     }
-    for (int i = 0; i < kBufs * kHalves; ++i) {
+    for (int i = 0; i < kBufs * kHalves; ++i)
       mbar_init(smem_u32(&bars->tmem_empty[i]), (PAIR ? 2 : 1) * kEpiWarps / kHalves);
-    }
     for (int i = 0; i < S::kSlots; ++i) {
       mbar_init(smem_u32(&bars->scale_full[i]), 2);
       mbar_init(smem_u32(&bars->scale_empty[i]), kEpiWarps);
@@ -276,9 +279,9 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
       // The whole warp runs the loop and one lane issues: operands that are the
       // same in every lane stay in uniform registers, where the MMA wants them.
       // Its chain of dependent instructions is what a short k-block waits for,
-      // so it holds little: descriptors and barrier addresses
-      // advance by additions, and one commit per k-block tells the producer
-      // that the stage is free and the epilogue that its accumulator is full.
+      // so it holds little: descriptors and barrier addresses advance by
+      // additions, and a k-block's last commit tells the producer that the
+      // stage is free and the epilogue that its accumulator is full.
       constexpr uint32_t idesc = idesc_e4m3(kTileM, kHalfN);
       const uint64_t desc_a = smem_desc_sw128(smem_u32(s_a), 16, 1024);
       const uint64_t desc_b = smem_desc_sw128(smem_u32(s_b), 16, 1024);
@@ -416,7 +419,9 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
     const int seg1 = kHalves == 2 ? 128 + 64 * half : seg0 + 64;
     const uint32_t scale_full = smem_u32(&bars->scale_full[0]), scale_empty = smem_u32(&bars->scale_empty[0]);
     // this lane's row scale, and the warp's column scales, in slot 0
-    const uint32_t scale_row = smem_u32(s_scale) + static_cast<uint32_t>((BVEC || kHalves == 2 ? 0 : col_half * 128) + quarter * 32 + lane) * 4u;
+    const uint32_t scale_row =
+        smem_u32(s_scale) +
+        static_cast<uint32_t>((BVEC || kHalves == 2 ? 0 : col_half * 128) + quarter * 32 + lane) * 4u;
     const uint32_t scale_col = smem_u32(s_scale) + 128u * 4u;
     griddep_wait();
     uint32_t stage = 0, phase = 0, buf = 0, slot = 0, slot_phase = 0;
@@ -442,8 +447,8 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
         // Two 32-column reads of TMEM alternate: one is in flight while the
         // other is used. Warps past the matrix's edge add up zeros rather than
         // branch: without branches the warp stays converged and the chunks in
-        // one piece of code (8192^3: 866 -> 848 cycles a k-block, with column
-        // scales 1559 -> 1342).
+        // one piece of code (866 -> 848 cycles a k-block, with column scales 1559
+        // -> 1342).
         uint32_t r[2][32];
         tmem_ld_32x32b_x32(taddr, r[0]);
         const float s = ld_shared_f32(scale_row + slot * (S::kSlotFloats * 4));
@@ -471,7 +476,8 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
           for (int j = 0; j < 16; j += 2) {
             uint64_t c0 = c < 2 ? s2 : s2_second, c1 = c0;
             if constexpr (BVEC) {
-              ld_shared_2x64(cols + static_cast<uint32_t>((c < 2 ? seg0 + c * 32 : seg1 + (c - 2) * 32) + 2 * j) * 4u, c0, c1);
+              const int col = (c < 2 ? seg0 + c * 32 : seg1 + (c - 2) * 32) + 2 * j;
+              ld_shared_2x64(cols + static_cast<uint32_t>(col) * 4u, c0, c1);
               c0 = mul2(s2, c0);
               c1 = mul2(s2, c1);
             }
@@ -529,10 +535,13 @@ struct BlockConfig {
 
 BlockConfig select_block_config(int64_t m, int64_t n) {
   const int sms = current_sm_count();
-  // 256 x 256 tiles on CTA pairs where they fill the GPU at least half, else
-  // 128 x 128 tiles on single CTAs.
-  const int64_t pairs = ((m + 255) / 256) * ((n + 255) / 256);
-  return pairs * 4 >= sms ? BlockConfig{true, 256} : BlockConfig{false, 128};
+  // 128 x 128 tiles on single CTAs while they fit one wave, else 256 x 256 tiles
+  // on CTA pairs (four of the small ones). 512 x 4096 x 4096, 128 small tiles:
+  // 13.2 us against 17.8 in pairs; 1031 x 2053 x 1999, 153 of them: 15.8 against
+  // 12.6; 2048^3, 256: 14.2 against 12.7. With a scale per column 18.3 / 28.6,
+  // 19.0 / 18.1 and 19.5 / 18.0.
+  const int64_t singles = ((m + 127) / 128) * ((n + 127) / 128);
+  return singles > sms ? BlockConfig{true, 256} : BlockConfig{false, 128};
 }
 
 template <typename Kern>
