@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kSkinnyThreads, 2)
   constexpr bool kGate = KIND != kBlock;
   constexpr int kElemsK = kGate ? 64 : 128;  // elements of K in a k-block (128 bytes)
   constexpr int kBufs = kGate ? 1 : S::kBufs;
-  constexpr uint32_t kTmemCols = kBufs * NT < 32 ? 32 : kBufs * NT;
+  constexpr uint32_t kTmemCols = kBufs * NT <= 32 ? 32 : (kBufs * NT <= 64 ? 64 : (kBufs * NT <= 128 ? 128 : 256));
   constexpr int kOutCols = kGate ? 64 : 128;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -422,14 +422,15 @@ __global__ void __launch_bounds__(kSkinnyThreads, 2)
       if (left <= 0) continue;
       const uint32_t off = part_addr + static_cast<uint32_t>(t * 128 + c) * 4u;
       float v[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
-      if (split == 1) {
-        add_partials<1, kGate>(off, v, u);
-      } else if (split == 2) {
-        add_partials<2, kGate>(off, v, u);
-      } else if (split == 4) {
-        add_partials<4, kGate>(off, v, u);
-      } else {
-        add_partials<8, kGate>(off, v, u);
+      switch (split) {
+        case 1: add_partials<1, kGate>(off, v, u); break;
+        case 2: add_partials<2, kGate>(off, v, u); break;
+        case 3: add_partials<3, kGate>(off, v, u); break;
+        case 4: add_partials<4, kGate>(off, v, u); break;
+        case 5: add_partials<5, kGate>(off, v, u); break;
+        case 6: add_partials<6, kGate>(off, v, u); break;
+        case 7: add_partials<7, kGate>(off, v, u); break;
+        default: add_partials<8, kGate>(off, v, u);
       }
       if constexpr (kGate) {
         const int dt = p.ab_bf16 ? CHOREO_DTYPE_BF16 : CHOREO_DTYPE_F16;
@@ -468,18 +469,24 @@ namespace choreo_impl {
 
 // Rows of X up to which the skinny kernel is used, and its token tile.
 constexpr int64_t kSkinnyRows = 128;
-inline int skinny_tokens(int64_t m) { return m <= 16 ? 16 : (m <= 32 ? 32 : (m <= 64 ? 64 : 128)); }
+inline int skinny_tokens(int64_t m) { return m <= 16 ? 16 : (m <= 32 ? 32 : (m <= 64 ? 64 : (m <= 96 ? 96 : 128))); }
 
-// CTAs per tile: the fewest (a power of two, at most a portable cluster) that
-// give nearly every SM one, with at least four k-blocks each. One full-length
-// CTA an SM keeps 110 KB in flight, which is enough for HBM; more pieces only
-// add starts and reductions (m = 1, 160 tiles of 64 k-blocks: 28.8 us unsplit,
-// 36.5 in 2, 42.6 in 8), fewer leave SMs idle (m = 16, 32 tiles of 80: 15.4 us
-// in 4, 13.1 in 8).
+// CTAs per tile: the most (at most a portable cluster) whose grid is resident at
+// once, with at least four k-blocks each. More pieces spread the weights more
+// evenly over the SMs and keep more loads in flight; a second wave costs as much
+// as the first. An SM holds two CTAs, but a cluster has to lie within one group
+// of SMs, which leaves places unused: measured on a B200, clusters of 3 and 4
+// still fit at 15/16 of the places, of 5 to 8 at 7/8 (3 CTAs a tile: 92 tiles
+// 15.0 us, 95 tiles 23.3, in 2 18.9; 8 a tile: 32 tiles 7.2, 34 tiles 11.7).
+// 64-k-block gates of one row, fewest against most pieces: 60 tiles 11.5 (in 2)
+// and 9.2 us (in 4), 42 tiles 9.2 (in 3) and 8.0 (in 6), 16 tiles 7.3 (in 4) and
+// 5.8 (in 8); 70 to 74 tiles are the exception, 11.8 in 2 against 13.0 in 3.
 inline int skinny_split(int64_t tiles, int64_t k_blocks, int sms) {
-  int split = 1;
-  while (split < 8 && tiles * split < sms - sms / 8 && k_blocks / (2 * split) >= 4) split *= 2;
-  return split;
+  for (int split = 8; split > 1; --split) {
+    const int sixteenths = split > 4 ? 14 : (split > 2 ? 15 : 16);
+    if (tiles * split * 16 <= 2 * static_cast<int64_t>(sms) * sixteenths && k_blocks / split >= 4) return split;
+  }
+  return 1;
 }
 
 template <int KIND, int NT>
@@ -513,6 +520,7 @@ int launch_skinny(const choreo_sm100::TwoMaps& tw, const CUtensorMap& tx, const 
     case 16: return launch_skinny_nt<KIND, 16>(tw, tx, kp, tiles, stream);
     case 32: return launch_skinny_nt<KIND, 32>(tw, tx, kp, tiles, stream);
     case 64: return launch_skinny_nt<KIND, 64>(tw, tx, kp, tiles, stream);
+    case 96: return launch_skinny_nt<KIND, 96>(tw, tx, kp, tiles, stream);
     default: return launch_skinny_nt<KIND, 128>(tw, tx, kp, tiles, stream);
   }
 }

@@ -222,6 +222,26 @@ def test_product_against_64_bits(cb, cuda, block_b, out):
         assert (c[m:] == 5.0).all() and (c[:, n:] == 5.0).all()
 
 
+@pytest.mark.parametrize("m", [1, 20, 64, 66, 96, 128])
+@pytest.mark.parametrize("block_b", [1, 128])
+def test_few_rows_in_every_number_of_pieces(cb, cuda, block_b, m):
+    import torch
+    seen = set()
+    for tiles, k in ((160, 200), (120, 1100), (80, 1600), (60, 2100), (45, 2700), (40, 3200), (35, 3800), (20, 4100)):
+        n = 128 * tiles - 3
+        a, sa = make_operand(cb, m, k, 10, 1)
+        b, sb = make_operand(cb, n, k, 90, block_b, std=k ** -0.5)
+        c = torch.full((m + 1, n), 5.0, device="cuda", dtype=torch.float32)
+        seen.add(cb.gemm_block_scaled_query(cb.gemm_block_desc(a, sa, b, sb, c[:m])).split_k)
+        cb.gemm_block_scaled(a, sa, b, sb, c[:m])
+        cb.sync_status()
+        want, bound = product_and_bound(a, sa, b, sb, block_b, torch.float32)
+        assert_within(c[:m], want, bound, (m, n, k))
+        assert (c[m:] == 5.0).all()
+    if torch.cuda.get_device_properties(0).multi_processor_count == 148:
+        assert seen == set(range(1, 9))
+
+
 @pytest.mark.parametrize("m,n,k", [(5, 300, 1000), (200, 264, 700), (1100, 1288, 900)])
 @pytest.mark.parametrize("out", ["bf16", "f32"])
 @pytest.mark.parametrize("block_b", [1, 128])

@@ -138,6 +138,32 @@ def test_forward(cb, cuda, trans, dt, act):
             assert untouched(gbuf, m, n) and untouched(ubuf, m, n)
 
 
+@pytest.mark.parametrize("m", [1, 5, 17, 50, 77, 96, 97, 128])
+@pytest.mark.parametrize("trans", [False, True])
+def test_few_rows_in_every_number_of_pieces(cb, cuda, trans, m):
+    """K is cut over one to eight CTAs, unevenly where it does not divide; a
+    rank may have no row of H to add up."""
+    seen = set()
+    for tiles, k in ((300, 100), (120, 700), (80, 1000), (60, 1300), (45, 1400), (40, 1610), (35, 1900), (20, 2100)):
+        n = 64 * tiles - 3
+        c = Case(m, n, k, "bf16", "silu", trans, seed=tiles)
+        h, hbuf = output(m, n, c.dt, 1)
+        seen.add(cb.gated_ffn_query(cb.ffn_desc(c.x, c.wg, c.wu, h, trans_w=trans)).split_k)
+        cb.gated_ffn(c.x, c.wg, c.wu, h, trans_w=trans)
+        cb.sync_status()
+        g, u, eg, eu = c.products()
+        want, e = c.hidden(g, u, eg, eu)
+        assert_within(h, want, e + rounding(want.abs() + e, c.dt), (m, tiles))
+        assert untouched(hbuf, m, n), (m, tiles)
+    if cuda_sms() == 148:
+        assert seen == set(range(1, 9))
+
+
+def cuda_sms():
+    import torch
+    return torch.cuda.get_device_properties(0).multi_processor_count
+
+
 @pytest.mark.parametrize("tile", ["wide256", "pair256", "single128"])
 @pytest.mark.parametrize("trans", [False, True])
 @pytest.mark.parametrize("act", ["silu", "gelu"])
