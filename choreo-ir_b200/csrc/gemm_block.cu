@@ -332,7 +332,7 @@ __device__ __forceinline__ void block_body(const CUtensorMap* tma_a, const CUten
       // ------------------------------------------------------- scale warps
       // Each k-block's scales go through a ring of shared-memory slots, so the
       // epilogue neither addresses nor waits for global memory: with one scale
-      // per 128 rows of B the products sa(row) sb(column half), 2 x 128; else
+      // per 128 rows of B the products sa(row) sb(128 columns), 2 x 128; else
       // the 128 row scales and the BN column scales. The two warps take half
       // of the rows and of the columns each, loaded kAhead blocks ahead.
       griddep_wait();

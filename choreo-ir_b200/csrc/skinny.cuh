@@ -2,7 +2,7 @@
 // reading the weights once, so the kernel is built around their stream.
 //
 // The weights are the MMA's 128-row operand and the tokens its NT columns
-// (NT = 16 .. 128), so no tensor work is spent on absent rows. One CTA streams
+// (NT = 16, 32, 64, 96 or 128), so little tensor work goes to absent rows. One CTA streams
 // 128 weight rows x 128 bytes per k-block; `split` CTAs of a cluster each take
 // a range of the k-blocks of one tile, so that a few tiles still keep every SM
 // loading, and add their partial sums through distributed shared memory in a
@@ -22,9 +22,9 @@
 // to fp32 sums in registers.
 //
 // Measured: 1 x 4096 x 10240 bf16 gate, weights N x K, 29.6 us = 0.86 of the
-// copy bandwidth (K x N: 25.9 us = 0.99); 16 x 10240 x 4096 in 8 bits 13.1 us
-// for 6.5 us of bytes, the rest the start of ten k-blocks a CTA and the
-// reduction over 8 CTAs.
+// copy bandwidth (K x N: 27.2 us = 0.94); 77 x 2056 x 5461 f16 gate 16.1 us for
+// 7 us of bytes, 16 x 10240 x 4096 in 8 bits 13.4 us for 6.5, the rest the start
+// of ten k-blocks a CTA and the reduction over the cluster.
 #pragma once
 #include <algorithm>
 
@@ -476,11 +476,13 @@ inline int skinny_tokens(int64_t m) { return m <= 16 ? 16 : (m <= 32 ? 32 : (m <
 // evenly over the SMs and keep more loads in flight; a second wave costs as much
 // as the first. An SM holds two CTAs, but a cluster has to lie within one group
 // of SMs, which leaves places unused: measured on a B200, clusters of 3 and 4
-// still fit at 15/16 of the places, of 5 to 8 at 7/8 (3 CTAs a tile: 92 tiles
-// 15.0 us, 95 tiles 23.3, in 2 18.9; 8 a tile: 32 tiles 7.2, 34 tiles 11.7).
-// 64-k-block gates of one row, fewest against most pieces: 60 tiles 11.5 (in 2)
-// and 9.2 us (in 4), 42 tiles 9.2 (in 3) and 8.0 (in 6), 16 tiles 7.3 (in 4) and
-// 5.8 (in 8); 70 to 74 tiles are the exception, 11.8 in 2 against 13.0 in 3.
+// still fit at 15/16 of the places, of 5 to 8 at 7/8 (weights in L2, 3 CTAs a
+// tile: 92 tiles 15.0 us, 95 tiles 23.3, in 2 18.9; 8 a tile: 32 tiles 7.2, 34
+// tiles 11.7). Weights from HBM, fewest against most pieces: 77 x 2056 x 5461
+// gate 19.8 us in 1, 16.1 in 3; 16 x 4096 x 4096 19.8 in 1, 15.1 in 4; 16 x
+// 10240 x 4096 in 8 bits 15.7 in 4, 13.4 in 8; 1 x 2048 x 5632 gate alike in 1
+// and 3 (11.5, 11.1; in L2 10.5, 8.4); the worst for the rule 6.5 in 4, 6.8 in 8
+// (1 x 2048 x 2048).
 inline int skinny_split(int64_t tiles, int64_t k_blocks, int sms) {
   for (int split = 8; split > 1; --split) {
     const int sixteenths = split > 4 ? 14 : (split > 2 ? 15 : 16);
