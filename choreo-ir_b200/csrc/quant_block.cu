@@ -5,8 +5,9 @@
 //   scale = a / 448,  q = e4m3(x * (448 / a)),  each step rounded to fp32
 //
 // Memory-bound: 2 or 4 bytes read and 1 written per element. 8192 x 10240 bf16
-// in rows 46 us = 0.84 of the copy bandwidth, transposed 55 us; 8191 x 4100 f32
-// in 128 x 128 blocks, transposed, 37 us = 0.69.
+// in rows 46 us = 0.84 of the copy bandwidth, transposed 49 us with either block;
+// f32 transposed 68 us (128 x 128) and 71 us (1 x 128) = 0.95 and 0.91; 8191 x
+// 4100 f32 in 128 x 128 blocks, transposed, 32 us = 0.80.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -28,7 +29,7 @@ struct QuantParams {
   int64_t ldq;
   float* scale;
   int64_t scale_row, scale_blk;
-  int32_t q_vec;               // 8-byte stores to q's rows are legal
+  int32_t q_vec;               // bytes (16, 8) that a store to q's rows may have, 0: one
 };
 
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
@@ -83,6 +84,8 @@ struct Piece {
           w[i / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + i)) << (16 * (i & 1));
       }
   }
+  // Magnitude bits of word j: of two 16-bit elements or of one of 32 bits.
+  __device__ __forceinline__ uint32_t top_of(int j) const { return w[j] & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu); }
   // Largest magnitude, as ordered bits: two 16-bit halves or one 32-bit value.
   __device__ __forceinline__ uint32_t top() const {
     if constexpr (sizeof(T) == 4) {
@@ -128,6 +131,20 @@ __device__ __forceinline__ void quantize_piece(const Piece<T>& v, float inv, boo
   if (!clean) {
 #pragma unroll
     for (int i = 0; i < Piece<T>::kElems; ++i) f[i] = finite_or_nan(v.get(i)) * inv;
+  }
+  q[0] = e4m3x4(f[0], f[1], f[2], f[3]);
+  if constexpr (sizeof(T) == 2) q[1] = e4m3x4(f[4], f[5], f[6], f[7]);
+}
+// The same with a factor of its own for each element.
+template <typename T>
+__device__ __forceinline__ void quantize_piece(const Piece<T>& v, const float (&inv)[Piece<T>::kElems], bool clean,
+                                               uint32_t (&q)[2]) {
+  float f[Piece<T>::kElems];
+#pragma unroll
+  for (int i = 0; i < Piece<T>::kElems; ++i) f[i] = v.get(i) * inv[i];
+  if (!clean) {
+#pragma unroll
+    for (int i = 0; i < Piece<T>::kElems; ++i) f[i] = finite_or_nan(v.get(i)) * inv[i];
   }
   q[0] = e4m3x4(f[0], f[1], f[2], f[3]);
   if constexpr (sizeof(T) == 2) q[1] = e4m3x4(f[4], f[5], f[6], f[7]);
@@ -242,143 +259,208 @@ __device__ __forceinline__ float cta_amax(uint32_t top, float finite_top, uint32
   return m;
 }
 
-// One 128 x 128 tile of op(X) per CTA. SQUARE: one scale for the tile, else one
-// per row of op(X).
-//
-// TRANS: the tile is loaded along X's rows (op(X)'s columns) and turned in
-// shared memory. There each row of op(X) is cut into 16-byte chunks (8 rows of
-// X, 4 for f32), chunk j of row c stored at j ^ (c / elements per load): a
-// warp's store touches 4 words of a chunk in 8 different chunks, its load of
-// whole chunks 8 different chunks per 8 lanes, both without bank conflicts.
-template <typename T, bool SQUARE, bool TRANS, int kThreads>
+// Largest finite magnitude of the CTA's pieces; *clean: no NaN or infinity.
+template <typename T, int kPieces, int kWarps>
+__device__ __forceinline__ float tile_amax(const Piece<T> (&v)[kPieces], uint32_t* warp_top, float* warp_finite,
+                                           bool* clean) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) top = top_max<T>(top, v[i].top());
+  bool own_clean;
+  float m = top_value<T>(top, &own_clean);
+  if (!own_clean) {
+    m = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) m = fmaxf(m, v[i].finite_top());
+  }
+  return cta_amax<T, kWarps>(top, m, warp_top, warp_finite, clean);
+}
+
+// One 128 x 128 tile of X per CTA with one scale, stored as it lies. Thread:
+// kPieces pieces of 16 bytes; a warp load takes 32 / kLanes whole tile rows.
+template <typename T, int kThreads>
 __global__ void __launch_bounds__(kThreads) quant_tile_kernel(const QuantParams p) {
   constexpr int kWarps = kThreads / 32;
-  constexpr int E = Piece<T>::kElems;        // elements of a load; rows of X in a chunk
+  constexpr int E = Piece<T>::kElems;
   constexpr int kPieces = 128 * 128 / E / kThreads;
   constexpr int kLanes = 128 / E;
-  constexpr int kWords = 128 * static_cast<int>(sizeof(T)) / 4;  // 32-bit words of a tile row
-  extern __shared__ uint4 turned_raw[];
-  uint32_t* turned = reinterpret_cast<uint32_t*>(turned_raw);
+  constexpr int kRows = 32 / kLanes;  // rows of one warp load
   __shared__ uint32_t warp_top[kWarps];
   __shared__ float warp_finite[kWarps];
   griddep_wait();
   griddep_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t rt = blockIdx.x / p.col_tiles, ct = blockIdx.x - rt * p.col_tiles;
-  const int64_t r0 = rt * 128, c0 = ct * 128;
+  const int64_t r0 = rt * 128, c = ct * 128 + lane % kLanes * E;
   const T* x = static_cast<const T*>(p.x);
   Piece<T> v[kPieces];
-  if constexpr (!TRANS) {
-    // piece i of the thread: row i * 8 * rows-per-warp + ..., kLanes lanes a row
-    constexpr int kRows = 32 / kLanes;  // rows of one warp load
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int64_t r = r0 + (i * kWarps + warp) * kRows + lane / kLanes;
-      const int64_t c = c0 + lane % kLanes * E;
-      v[i].load(x + (r < p.rows ? r : p.rows - 1) * p.ldx + c, r < p.rows ? p.cols - c : 0);
-    }
-  } else {
-    // A warp load covers 8 pieces of 4 rows of X: 4 words (row pairs for 16
-    // bits) of one chunk. 16-bit loads come in pairs of rows.
-    constexpr int kGroups = kLanes / 8;      // 8-piece groups across the tile
-    constexpr int kPair = 4 / static_cast<int>(sizeof(T)) ;  // rows of X in one word
-#pragma unroll
-    for (int i = 0; i < kPieces / kPair; ++i) {
-      const int unit = i * kWarps + warp;    // (chunk, group)
-      const int chunk = unit / kGroups, grp = unit % kGroups;
-#pragma unroll
-      for (int h = 0; h < kPair; ++h) {
-        const int64_t k = c0 + chunk * E + (lane >> 3) * kPair + h;  // row of X
-        const int64_t r = r0 + (grp * 8 + (lane & 7)) * E;           // column of X
-        v[i * kPair + h].load(x + (k < p.cols ? k : p.cols - 1) * p.ldx + r, k < p.cols ? p.rows - r : 0);
-      }
-    }
+  for (int i = 0; i < kPieces; ++i) {
+    const int64_t r = r0 + (i * kWarps + warp) * kRows + lane / kLanes;
+    v[i].load(x + (r < p.rows ? r : p.rows - 1) * p.ldx + c, r < p.rows ? p.cols - c : 0);
   }
-  float inv = 0.f;
+  bool clean;
+  const float amax = tile_amax<T, kPieces, kWarps>(v, warp_top, warp_finite, &clean);
+  const float inv = factor_of(amax);
+  if (threadIdx.x == 0) p.scale[rt * p.scale_row + ct * p.scale_blk] = scale_of(amax);
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    const int64_t r = r0 + (i * kWarps + warp) * kRows + lane / kLanes;
+    if (r >= p.rows) continue;
+    uint32_t q[2];
+    quantize_piece<T>(v[i], inv, clean, q);
+    store_q<E>(p.q + r * p.ldq + c, q, p.cols - c, p.q_vec != 0);
+  }
+}
+
+// One 128 x 128 tile of X per CTA, turned: rows of X are columns of op(X).
+// SQUARE: one scale for the tile, else one per column of X.
+//
+// A thread loads the same columns of X (16 bytes) in groups of four rows, so a
+// warp load covers whole tile rows, the largest value of a column is a maximum
+// over registers and then over the warps, and four rows' codes of a column are
+// one word after a 4 x 4 byte transpose. Only codes go through shared memory (16
+// KB, not the tile's 32 or 64). There word g (rows 4 g .. of X) of column c
+// stands at g ^ (c / E * E / 4): the lanes of a store, at neighbouring c / E,
+// meet 32 banks, and a 16-byte load still finds its four words in one chunk, in
+// an order that depends on the column only. 8 lanes write one 128-byte row.
+//
+// Turning the elements and quantising afterwards, as this kernel did first, took
+// 76 and 96 us for f32 and 50 and 56 us for bf16 at 8192 x 10240: its tile filled
+// 64 KB, and a 1 x 128 block cost shuffles over 16 or 32 lanes. Three CTAs an SM
+// for f32 (2: 76 us, 4 spills: 85), four for 16 bits (5: 46 us here but 8.5
+// against 7.9 at 4096 x 2048, 3: 53, 6 spills).
+template <typename T, bool SQUARE, int kMinCtas>
+__global__ void __launch_bounds__(256, kMinCtas) quant_turn_kernel(const QuantParams p) {
+  constexpr int kWarps = 8;
+  constexpr int E = Piece<T>::kElems;
+  constexpr int kLanes = 128 / E;
+  constexpr int kSteps = kLanes / kWarps;  // groups of four rows a thread takes
+  __shared__ uint4 turned_raw[128 * 8];
+  __shared__ uint4 warp_cols[kWarps][SQUARE ? 1 : kLanes];  // each warp's column maxima, as top bits
+  __shared__ float col_inv[SQUARE ? 1 : 128];
+  __shared__ uint32_t warp_top[kWarps];
+  __shared__ float warp_finite[kWarps];
+  uint32_t* turned = reinterpret_cast<uint32_t*>(turned_raw);
+  griddep_wait();
+  griddep_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, piece = lane % kLanes;
+  const int64_t rt = blockIdx.x / p.col_tiles, ct = blockIdx.x - rt * p.col_tiles;
+  const int64_t r0 = rt * 128, c0 = ct * 128;  // row and column of op(X): column and row of X
+  const T* x = static_cast<const T*>(p.x);
+  auto group_of = [&](int s) { return (s * kWarps + warp) * (32 / kLanes) + lane / kLanes; };
+  Piece<T> v[kSteps * 4];
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const int64_t k = c0 + group_of(s) * 4 + h;
+      const int64_t r = r0 + piece * E;
+      v[s * 4 + h].load(x + (k < p.cols ? k : p.cols - 1) * p.ldx + r, k < p.cols ? p.rows - r : 0);
+    }
   bool clean = true;
+  float inv[SQUARE ? 1 : E];
   if constexpr (SQUARE) {
-    uint32_t top = 0;
-    float m = 0.f;
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      top = top_max<T>(top, v[i].top());
-    }
-    bool own_clean;
-    m = top_value<T>(top, &own_clean);
-    if (!own_clean) {
-      m = 0.f;
-#pragma unroll
-      for (int i = 0; i < kPieces; ++i) m = fmaxf(m, v[i].finite_top());
-    }
-    const float amax = cta_amax<T, kWarps>(top, m, warp_top, warp_finite, &clean);
-    inv = factor_of(amax);
+    const float amax = tile_amax<T, kSteps * 4, kWarps>(v, warp_top, warp_finite, &clean);
+    inv[0] = factor_of(amax);
     if (threadIdx.x == 0) p.scale[rt * p.scale_row + ct * p.scale_blk] = scale_of(amax);
-  }
-  if constexpr (!TRANS) {
-    static_assert(TRANS || SQUARE, "rows of X as they lie are quant_rows_kernel's");
-    constexpr int kRows = 32 / kLanes;
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int64_t r = r0 + (i * kWarps + warp) * kRows + lane / kLanes;
-      const int64_t c = c0 + lane % kLanes * E;
-      if (r >= p.rows) continue;
-      uint32_t q[2];
-      quantize_piece<T>(v[i], inv, clean, q);
-      store_q<E>(p.q + r * p.ldq + c, q, p.cols - c, p.q_vec != 0);
-    }
   } else {
-    constexpr int kGroups = kLanes / 8;
-    constexpr int kPair = 4 / static_cast<int>(sizeof(T));
+    uint32_t top[4];
 #pragma unroll
-    for (int i = 0; i < kPieces / kPair; ++i) {
-      const int unit = i * kWarps + warp;
-      const int chunk = unit / kGroups, grp = unit % kGroups;
-      const int piece = grp * 8 + (lane & 7);  // columns of X piece * E .. + E - 1
-      uint32_t* dst = turned + piece * E * kWords + ((chunk ^ piece) * 4 + (lane >> 3));
+    for (int j = 0; j < 4; ++j) {
+      top[j] = v[0].top_of(j);
+#pragma unroll
+      for (int i = 1; i < kSteps * 4; ++i) top[j] = top_max<T>(top[j], v[i].top_of(j));
+      if (kLanes == 16) top[j] = top_max<T>(top[j], __shfl_xor_sync(0xffffffffu, top[j], 16));
+    }
+    if (lane < kLanes) warp_cols[warp][lane] = make_uint4(top[0], top[1], top[2], top[3]);
+    __syncthreads();
+    // Thread c finishes column c.
+    const int c = threadIdx.x;
+    float amax = 0.f;
+    bool finite = true;
+    if (c < 128) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const uint32_t word = reinterpret_cast<const uint32_t*>(warp_cols[w])[sizeof(T) == 4 ? c : c / 2];
+        m = max(m, sizeof(T) == 4 ? word : ((c & 1) ? word >> 16 : word & 0xffffu));
+      }
+      amax = top_value<T>(m, &finite);
+    }
+    clean = __syncthreads_or(finite ? 0 : 1) == 0;
+    if (!clean) {  // NaN or an infinity in the tile: the columns' largest finite values
+      float* fin = reinterpret_cast<float*>(turned);  // [warp][column]
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        uint32_t w;
-        if constexpr (sizeof(T) == 4)
-          w = v[i].w[e];
-        else
-          w = __byte_perm(v[2 * i].w[e / 2], v[2 * i + 1].w[e / 2], (e & 1) ? 0x7632 : 0x5410);
-        dst[e * kWords] = w;
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < kSteps * 4; ++i) m = fmaxf(m, finite_abs(v[i].get(e)));
+        if (kLanes == 16) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+        if (lane < kLanes) fin[warp * 128 + piece * E + e] = m;
       }
+      __syncthreads();
+      if (c < 128) {
+        amax = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) amax = fmaxf(amax, fin[w * 128 + c]);
+      }
+      // (the barrier below also separates these reads from the codes' stores)
+    }
+    if (c < 128) {
+      col_inv[c] = factor_of(amax);
+      if (r0 + c < p.rows) p.scale[(r0 + c) * p.scale_row + ct * p.scale_blk] = scale_of(amax);
     }
     __syncthreads();
-    constexpr int kRows = 32 / kLanes;  // rows of op(X) of one warp load
-    constexpr int kSteps = 128 / kWarps / kRows;
-    constexpr int kStep = kSteps < 4 ? kSteps : 4;  // rows in registers at once
-    const int part = lane % kLanes;
-    const int64_t c = c0 + part * E;
-#pragma unroll 1
-    for (int i0 = 0; i0 < kSteps; i0 += kStep) {
-      auto row_of = [&](int i) { return ((i0 + i) * kWarps + warp) * kRows + lane / kLanes; };
-      Piece<T> u[kStep];
-      float amax[kStep];
-      bool ok[kStep];
 #pragma unroll
-      for (int i = 0; i < kStep; ++i) {
-        const int row = row_of(i);
-        const uint4 w = *reinterpret_cast<const uint4*>(turned + row * kWords + (part ^ (row / E)) * 4);
-        u[i].w[0] = w.x, u[i].w[1] = w.y, u[i].w[2] = w.z, u[i].w[3] = w.w;
-        ok[i] = clean;
-        if constexpr (!SQUARE) amax[i] = group_amax<T, kLanes>(u[i], &ok[i]);
-      }
-      if constexpr (!SQUARE) {
-        const float own = pick<kStep>(amax, part % kStep);
-        inv = factor_of(own);
-        const int64_t r = r0 + row_of(part);
-        if (part < kStep && r < p.rows) p.scale[r * p.scale_row + ct * p.scale_blk] = scale_of(own);
-      }
+    for (int e = 0; e < E; ++e) inv[e] = col_inv[piece * E + e];
+  }
 #pragma unroll
-      for (int i = 0; i < kStep; ++i) {
-        const int64_t r = r0 + row_of(i);
-        const float f = SQUARE ? inv : __shfl_sync(0xffffffffu, inv, (lane & ~(kLanes - 1)) | i);
-        uint32_t q[2];
-        quantize_piece<T>(u[i], f, ok[i], q);
-        if (r < p.rows) store_q<E>(p.q + r * p.ldq + c, q, p.cols - c, p.q_vec != 0);
-      }
+  for (int s = 0; s < kSteps; ++s) {
+    uint32_t q[4][2];
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      if constexpr (SQUARE)
+        quantize_piece<T>(v[s * 4 + h], inv[0], clean, q[h]);
+      else
+        quantize_piece<T>(v[s * 4 + h], inv, clean, q[h]);
+    }
+    uint32_t* dst = turned + piece * E * 32 + (group_of(s) ^ (piece * (E / 4)));
+#pragma unroll
+    for (int b = 0; b < E / 4; ++b) {  // columns 4 b .. 4 b + 3 of the piece
+      const uint32_t lo01 = __byte_perm(q[0][b], q[1][b], 0x5140), lo23 = __byte_perm(q[2][b], q[3][b], 0x5140);
+      const uint32_t hi01 = __byte_perm(q[0][b], q[1][b], 0x7362), hi23 = __byte_perm(q[2][b], q[3][b], 0x7362);
+      dst[(4 * b + 0) * 32] = __byte_perm(lo01, lo23, 0x5410);
+      dst[(4 * b + 1) * 32] = __byte_perm(lo01, lo23, 0x7632);
+      dst[(4 * b + 2) * 32] = __byte_perm(hi01, hi23, 0x5410);
+      dst[(4 * b + 3) * 32] = __byte_perm(hi01, hi23, 0x7632);
+    }
+  }
+  __syncthreads();
+  const int part = lane & 7;  // 16 columns of op(X)
+  const int64_t left = p.cols - c0 - part * 16;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = (i * kWarps + warp) * 4 + (lane >> 3);
+    const int turn = row / E * (E / 4);
+    const uint4 w = turned_raw[row * 8 + (part ^ (turn >> 2))];
+    uint32_t a = w.x, b = w.y, c = w.z, d = w.w;
+    if (turn & 1) {
+      const uint32_t a0 = a, c0s = c;
+      a = b, b = a0, c = d, d = c0s;
+    }
+    if (turn & 2) {
+      const uint32_t a0 = a, b0 = b;
+      a = c, c = a0, b = d, d = b0;
+    }
+    if (r0 + row >= p.rows || left <= 0) continue;
+    uint8_t* q = p.q + (r0 + row) * p.ldq + c0 + part * 16;
+    if (left >= 16 && p.q_vec == 16) {
+      *reinterpret_cast<uint4*>(q) = make_uint4(a, b, c, d);
+    } else {
+      const uint32_t first[2] = {a, b}, second[2] = {c, d};
+      store_q<8>(q, first, left, p.q_vec != 0);
+      store_q<8>(q + 8, second, left - 8, p.q_vec != 0);
     }
   }
 }
@@ -477,8 +559,10 @@ int launch_tile(const QuantParams& p, bool x_vec, cudaStream_t s) {
   if constexpr (SQUARE || TRANS) {
     static std::atomic<uint64_t> done{0};
     constexpr int kThreads = 256;
-    return launch_quant(quant_tile_kernel<T, SQUARE, TRANS, kThreads>, grid, kThreads,
-                        TRANS ? 128 * 128 * static_cast<int>(sizeof(T)) : 0, done, s, p);
+    if constexpr (TRANS)
+      return launch_quant(quant_turn_kernel<T, SQUARE, sizeof(T) == 4 ? 3 : 4>, grid, 256, 0, done, s, p);
+    else
+      return launch_quant(quant_tile_kernel<T, kThreads>, grid, kThreads, 0, done, s, p);
   } else {
     // Four loads in flight a thread where that still leaves every SM two CTAs;
     // a few rows are spread over as many SMs as one load each can reach.
@@ -536,7 +620,8 @@ extern "C" int choreo_quantize_block(const choreo_quant_desc* d, void* stream) {
   p.col_tiles = col_blocks;
   const bool x_vec =
       ((reinterpret_cast<uintptr_t>(d->x) | static_cast<uintptr_t>(d->ldx * dtype_bytes(d->dtype))) & 15u) == 0;
-  p.q_vec = ((reinterpret_cast<uintptr_t>(d->q) | static_cast<uintptr_t>(d->ldq)) & 7u) == 0;
+  const uintptr_t q_bits = reinterpret_cast<uintptr_t>(d->q) | static_cast<uintptr_t>(d->ldq);
+  p.q_vec = (q_bits & 15u) == 0 ? 16 : ((q_bits & 7u) == 0 ? 8 : 0);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool rows = d->block_rows == 1, trans = d->transpose != 0;
   switch (d->dtype) {
