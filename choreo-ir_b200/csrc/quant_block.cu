@@ -5,9 +5,9 @@
 //   scale = a / 448,  q = e4m3(x * (448 / a)),  each step rounded to fp32
 //
 // Memory-bound: 2 or 4 bytes read and 1 written per element. 8192 x 10240 bf16
-// in rows 46 us = 0.84 of the copy bandwidth, transposed 49 us with either block;
-// f32 transposed 68 us (128 x 128) and 71 us (1 x 128) = 0.95 and 0.91; 8191 x
-// 4100 f32 in 128 x 128 blocks, transposed, 32 us = 0.80.
+// in rows 46 us = 0.84 of the copy bandwidth, transposed 48 us with either block;
+// f32 transposed 65 us (128 x 128) and 68 us (1 x 128) = 0.98 and 0.94; 8191 x
+// 4100 f32 in 128 x 128 blocks, transposed, 31.5 us = 0.81.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -345,7 +345,8 @@ __global__ void __launch_bounds__(256, kMinCtas) quant_turn_kernel(const QuantPa
   griddep_wait();
   griddep_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, piece = lane % kLanes;
-  const int64_t rt = blockIdx.x / p.col_tiles, ct = blockIdx.x - rt * p.col_tiles;
+  // Neighbouring CTAs read neighbouring columns of X (2 to 4 % over the other order).
+  const int64_t ct = blockIdx.x / p.row_tiles, rt = blockIdx.x - ct * p.row_tiles;
   const int64_t r0 = rt * 128, c0 = ct * 128;  // row and column of op(X): column and row of X
   const T* x = static_cast<const T*>(p.x);
   auto group_of = [&](int s) { return (s * kWarps + warp) * (32 / kLanes) + lane / kLanes; };
