@@ -303,11 +303,7 @@ int choreo_gated_ffn_query(const choreo_ffn_desc* d, choreo_launch_config* out) 
     out->tiles *= out->split_k;
     out->grid_x = static_cast<int32_t>(out->tiles);
     out->block_x = kSkinnyThreads;
-    out->stages = nt == 16 ? SkinnyShape<16>::kStages : nt == 32 ? SkinnyShape<32>::kStages
-                : nt == 64 ? SkinnyShape<64>::kStages : SkinnyShape<128>::kStages;
-    out->smem_bytes = nt == 16 ? SkinnyShape<16>::kSmem : nt == 32 ? SkinnyShape<32>::kSmem
-                    : nt == 64 ? SkinnyShape<64>::kSmem : SkinnyShape<128>::kSmem;
-    out->tmem_cols = std::max(nt, 32);
+    skinny_shape(nt, true, out);
     return ok();
   }
   const TcConfig c = select_gate_config(d->m, d->n, d->k);

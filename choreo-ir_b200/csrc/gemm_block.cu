@@ -699,11 +699,7 @@ int choreo_gemm_block_scaled_query(const choreo_gemm_block_desc* d, choreo_launc
     out->tiles *= out->split_k;
     out->grid_x = static_cast<int32_t>(out->tiles);
     out->block_x = kSkinnyThreads;
-    out->stages = nt == 16 ? SkinnyShape<16>::kStages : nt == 32 ? SkinnyShape<32>::kStages
-                : nt == 64 ? SkinnyShape<64>::kStages : SkinnyShape<128>::kStages;
-    out->smem_bytes = nt == 16 ? SkinnyShape<16>::kSmem : nt == 32 ? SkinnyShape<32>::kSmem
-                    : nt == 64 ? SkinnyShape<64>::kSmem : SkinnyShape<128>::kSmem;
-    out->tmem_cols = nt * (nt <= 64 ? 4 : 2);
+    skinny_shape(nt, false, out);
     return ok();
   }
   const BlockConfig c = select_block_config(d->m, d->n);

@@ -149,6 +149,8 @@ __device__ __forceinline__ void act_quad(int act, float (&g)[4]) {
   }
 }
 
+constexpr uint32_t skinny_tmem_cols(int used) { return used <= 32 ? 32 : (used <= 64 ? 64 : (used <= 128 ? 128 : 256)); }
+
 template <int NT>
 struct SkinnyShape {
   static constexpr uint32_t kWStage = 128 * 128;  // bytes: 128 rows x 128 bytes of K
@@ -180,7 +182,7 @@ __global__ void __launch_bounds__(kSkinnyThreads, 2)
   constexpr bool kGate = KIND != kBlock;
   constexpr int kElemsK = kGate ? 64 : 128;  // elements of K in a k-block (128 bytes)
   constexpr int kBufs = kGate ? 1 : S::kBufs;
-  constexpr uint32_t kTmemCols = kBufs * NT <= 32 ? 32 : (kBufs * NT <= 64 ? 64 : (kBufs * NT <= 128 ? 128 : 256));
+  constexpr uint32_t kTmemCols = skinny_tmem_cols(kBufs * NT);
   constexpr int kOutCols = kGate ? 64 : 128;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -489,6 +491,24 @@ inline int skinny_split(int64_t tiles, int64_t k_blocks, int sms) {
     if (tiles * split * 16 <= 2 * static_cast<int64_t>(sms) * sixteenths && k_blocks / split >= 4) return split;
   }
   return 1;
+}
+
+template <int NT>
+void skinny_shape_nt(bool gate, choreo_launch_config* out) {
+  using S = choreo_sm100::SkinnyShape<NT>;
+  out->stages = S::kStages;
+  out->smem_bytes = S::kSmem;
+  out->tmem_cols = static_cast<int32_t>(choreo_sm100::skinny_tmem_cols(NT * (gate ? 1 : S::kBufs)));
+}
+// What a query reports of the kernel for `nt` tokens.
+inline void skinny_shape(int nt, bool gate, choreo_launch_config* out) {
+  switch (nt) {
+    case 16: return skinny_shape_nt<16>(gate, out);
+    case 32: return skinny_shape_nt<32>(gate, out);
+    case 64: return skinny_shape_nt<64>(gate, out);
+    case 96: return skinny_shape_nt<96>(gate, out);
+    default: return skinny_shape_nt<128>(gate, out);
+  }
 }
 
 template <int KIND, int NT>

@@ -317,6 +317,44 @@ def test_product_repeats_bit_for_bit_in_a_graph(cb, cuda, m, n, k):
         assert torch.equal(c, ref)
 
 
+@pytest.mark.parametrize("m", [100, 300])
+def test_offsets_past_32_bits(cb, cuda, m):
+    """Rows 2^23 elements apart, of the values, codes, scales and outputs."""
+    import torch
+    n, k, ld = 264, 500, 1 << 23
+    x = torch.randn(300, k, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+    floats = torch.empty(300, ld, device="cuda")
+    codes = torch.empty(k, ld, dtype=torch.uint8, device="cuda")
+    floats[:, :k] = x
+    for block, trans in ((1, False), (128, False), (1, True), (128, True)):
+        r, c = (k, 300) if trans else (300, k)
+        q, want_q = codes[:r, :c].view(torch.float8_e4m3fn), torch.empty(r, -(-c // 16) * 16, dtype=torch.uint8, device="cuda")
+        want_q = want_q[:, :c].view(torch.float8_e4m3fn)
+        rows = -(-r // block)
+        scale = floats[:rows, 1024:1024 + -(-c // 128)] if rows <= 300 else torch.empty(rows, -(-c // 128), device="cuda")
+        want_s = torch.empty(rows, -(-c // 128), device="cuda")
+        cb.quantize_block(floats[:, :k], q, scale, block_rows=block, transpose=trans)
+        cb.quantize_block(x, want_q, want_s, block_rows=block, transpose=trans)
+        cb.sync_status()
+        assert torch.equal(scale, want_s) and torch.equal(q.contiguous().view(torch.uint8), want_q.contiguous().view(torch.uint8))
+    for block_b in (1, 128):
+        a, sa = make_operand(cb, m, k, 1, 1)
+        b, sb = make_operand(cb, n, k, 2, block_b)
+        addend = torch.randn(m, n, device="cuda")
+        fa, fb = codes[:m, :k], codes[:n, 1024:1024 + k]
+        fa.copy_(a.view(torch.uint8))
+        fb.copy_(b.view(torch.uint8))
+        fsa, fsb = floats[:m, 2048:2052], floats[:sb.shape[0], 2064:2068]
+        fsa.copy_(sa)
+        fsb.copy_(sb)
+        d, c, near = floats[:m, 4096:4096 + n], floats[:m, 8192:8192 + n], torch.empty(m, n, device="cuda")
+        d.copy_(addend)
+        cb.gemm_block_scaled(fa.view(torch.float8_e4m3fn), fsa, fb.view(torch.float8_e4m3fn), fsb, c, beta=2.0, addend=d)
+        cb.gemm_block_scaled(a, sa, b, sb, near, beta=2.0, addend=addend)
+        cb.sync_status()
+        assert torch.equal(c, near)
+
+
 def test_quantize_then_product(cb, cuda):
     """The three products of a linear layer in 8 bits: forward, input gradient
     (the weight quantised transposed) and weight gradient (both operands along

@@ -148,7 +148,11 @@ def test_few_rows_in_every_number_of_pieces(cb, cuda, trans, m):
         n = 64 * tiles - 3
         c = Case(m, n, k, "bf16", "silu", trans, seed=tiles)
         h, hbuf = output(m, n, c.dt, 1)
-        seen.add(cb.gated_ffn_query(cb.ffn_desc(c.x, c.wg, c.wu, h, trans_w=trans)).split_k)
+        q = cb.gated_ffn_query(cb.ffn_desc(c.x, c.wg, c.wu, h, trans_w=trans))
+        seen.add(q.split_k)
+        # a ring of `stages` k-blocks of 128 weight rows and tile_m tokens, 128 bytes each, and under 2 KB besides
+        assert m <= q.tile_m <= 128 and q.tmem_cols == max(32, 1 << (q.tile_m - 1).bit_length())
+        assert 0 < q.smem_bytes - q.stages * (128 + q.tile_m) * 128 < 2048
         cb.gated_ffn(c.x, c.wg, c.wu, h, trans_w=trans)
         cb.sync_status()
         g, u, eg, eu = c.products()
@@ -336,6 +340,43 @@ def test_special_values(cb, cuda):
             cb.sync_status()
             rows = torch.arange(m, device="cuda") == 2
             assert torch.isnan(h[2]).all() and torch.equal(h[~rows], ref[~rows])
+
+
+@pytest.mark.parametrize("m", [100, 300])
+@pytest.mark.parametrize("trans", [False, True])
+def test_offsets_past_32_bits(cb, cuda, m, trans):
+    """Every matrix a column window of one buffer whose rows lie 2^23 elements
+    apart: row 256 starts at 2^31."""
+    import torch
+    n, k, ld = 264, 296, 1 << 23
+    c = Case(m, n, k, "bf16", "silu", trans)
+    buf = torch.empty(300, ld, device="cuda", dtype=torch.bfloat16)
+    used = [0]
+
+    def window(rows, cols, src=None):
+        v = buf[:rows, used[0]:used[0] + cols]
+        used[0] += 512
+        if src is not None:
+            v.copy_(src)
+        return v
+
+    def far(src):
+        return window(*src.shape, src)
+
+    x, wg, wu, dh = far(c.x), far(c.wg), far(c.wu), far(c.dh)
+    h, gate, up, dx = window(m, n), window(m, n), window(m, n), window(m, k)
+    dwg, dwu = window(*wg.shape), window(*wg.shape)
+    near = [torch.empty(*v.shape, device="cuda", dtype=torch.bfloat16) for v in (h, gate, up, dx, dwg, dwu)]
+    cb.gated_ffn(x, wg, wu, h, trans_w=trans, gate=gate, up=up)
+    cb.gated_ffn(c.x, c.wg, c.wu, near[0], trans_w=trans, gate=near[1], up=near[2])
+    for kept in (False, True):
+        cb.gated_ffn_backward(dh, x, wg, wu, dx=dx, dw_gate=dwg, dw_up=dwu, trans_w=trans,
+                              **({"gate": gate, "up": up} if kept else {}))
+        cb.gated_ffn_backward(c.dh, c.x, c.wg, c.wu, dx=near[3], dw_gate=near[4], dw_up=near[5], trans_w=trans,
+                              **({"gate": near[1], "up": near[2]} if kept else {}))
+        cb.sync_status()
+        for got, want in zip((h, gate, up, dx, dwg, dwu), near):
+            assert torch.equal(got, want)
 
 
 def test_strides_shared_weight_matrix(cb, cuda):
