@@ -574,6 +574,7 @@ int dispatch_block(const BlockConfig& c, const CUtensorMap& ta, const CUtensorMa
 }
 
 int encode_e4m3(CUtensorMap* map, const void* p, int64_t rows, int64_t k, int64_t ld, uint32_t box_rows) {
+  if (rows == 1) ld = round_up(k, 16);  // never stepped over, but a map's stride has to be whole 16 bytes
   const uint64_t dims[3] = {static_cast<uint64_t>(k), static_cast<uint64_t>(rows), 1};
   const uint64_t strides[2] = {static_cast<uint64_t>(ld), static_cast<uint64_t>(rows) * static_cast<uint64_t>(ld)};
   const uint32_t box[3] = {kBlockK, box_rows, 1};
@@ -598,7 +599,8 @@ int validate_block(const choreo_gemm_block_desc* d) {
   if (d->lda < d->k || d->ldb < d->k)
     return fail(CHOREO_ERR_INVALID_ARG, "%s: lda=%lld or ldb=%lld smaller than K=%lld", what, (long long)d->lda,
                 (long long)d->ldb, (long long)d->k);
-  if (d->lda % 16 != 0 || d->ldb % 16 != 0 || (reinterpret_cast<uintptr_t>(d->a) & 15u) != 0 ||
+  // (a single row has no leading dimension to speak of)
+  if ((d->m > 1 && d->lda % 16 != 0) || (d->n > 1 && d->ldb % 16 != 0) || (reinterpret_cast<uintptr_t>(d->a) & 15u) != 0 ||
       (reinterpret_cast<uintptr_t>(d->b) & 15u) != 0)
     return fail(CHOREO_ERR_INVALID_ARG,
                 "%s: A, B and their leading dimensions must be multiples of 16 bytes (lda=%lld, ldb=%lld)", what,

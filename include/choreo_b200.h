@@ -395,8 +395,9 @@ int choreo_quantize_block(const choreo_quant_desc* d, void* stream);
  *   S[i,j] = sum over blocks t of scale_a(i, t) * scale_b(j, t)
  *            * sum over k in block t of A[i,k] * B[j,k]
  * A is M x K and B is N x K, e4m3, both K-contiguous (lda, ldb >= K and, like
- * the base addresses, multiples of 16 bytes: choreo_quantize_block makes both,
- * transposed where an operand is stored the other way round); blocks are 128
+ * the base addresses, multiples of 16 bytes unless there is a single row:
+ * choreo_quantize_block makes both, transposed where an operand is stored the
+ * other way round); blocks are 128
  * long along K (the last one may be shorter). scale_a(i, t) =
  * scale_a[i * scale_a_row + t * scale_a_blk]; scale_b(j, t) =
  * scale_b[(j / block_b) * scale_b_row + t * scale_b_blk], block_b 1 or 128.

@@ -317,6 +317,23 @@ def test_product_repeats_bit_for_bit_in_a_graph(cb, cuda, m, n, k):
         assert torch.equal(c, ref)
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 200, 1001), (150, 1, 333), (1, 1, 5)])
+def test_product_of_a_single_row(cb, cuda, m, n, k):
+    """One row's length is free: it starts on a 16-byte boundary by itself."""
+    import torch
+    a, sa = make_operand(cb, m, k, 1, 1)
+    b, sb = make_operand(cb, n, k, 2, 1)
+    if m == 1:
+        a = a.view(torch.uint8).flatten().clone().view(1, k)
+    if n == 1:
+        b = b.view(torch.uint8).flatten().clone().view(1, k)
+    c = torch.empty(m, n, device="cuda")
+    cb.gemm_block_scaled(a, sa, b, sb, c)
+    cb.sync_status()
+    want, bound = product_and_bound(a.view(torch.float8_e4m3fn), sa, b.view(torch.float8_e4m3fn), sb, 1, torch.float32)
+    assert_within(c, want, bound, (m, n, k))
+
+
 @pytest.mark.parametrize("m", [100, 300])
 def test_offsets_past_32_bits(cb, cuda, m):
     """Rows 2^23 elements apart, of the values, codes, scales and outputs."""
