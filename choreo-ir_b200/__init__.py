@@ -601,6 +601,8 @@ def gemm_block_desc(a, scale_a, b, scale_b, c, *, alpha=1.0, beta=0.0, addend=No
     n = b.shape[0]
     blocks = -(-k // 128)
     block_b = 1 if scale_b.shape[0] == n else 128
+    if bias is not None and (bias.shape != (n,) or not bias.is_contiguous()):
+        raise ValueError(f"bias: expected {n} contiguous elements, got {tuple(bias.shape)}")
     return GemmBlockDesc(m, n, k, a.data_ptr(), _e4m3_matrix(a, m, k, "a"), scale_a.data_ptr(),
                          *_scales(scale_a, m, blocks, "scale_a"), b.data_ptr(), _e4m3_matrix(b, n, k, "b"),
                          scale_b.data_ptr(), *_scales(scale_b, -(-n // block_b), blocks, "scale_b"), block_b,

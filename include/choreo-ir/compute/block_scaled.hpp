@@ -29,8 +29,12 @@ struct BlockScaled {
   Tensor<float> scales;            // ceil(cols / 128) x ceil(rows / block_rows)
 
   BlockScaled(index_t r, index_t c, index_t block)
-      : rows(r), cols(c), block_rows(block), codes(Shape({r, (c + 15) / 16 * 16}), MemoryType::DEVICE),
+      : rows(r), cols(c), block_rows(checked(block)), codes(Shape({r, (c + 15) / 16 * 16}), MemoryType::DEVICE),
         scales(Shape({(c + 127) / 128, (r + block - 1) / block}), MemoryType::DEVICE) {}
+  static index_t checked(index_t block) {
+    if (block != 1 && block != 128) throw ValidationError("BlockScaled: block_rows must be 1 or 128");
+    return block;
+  }
   index_t ld() const { return (cols + 15) / 16 * 16; }
   index_t row_blocks() const { return (rows + block_rows - 1) / block_rows; }
 };

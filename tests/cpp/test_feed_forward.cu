@@ -152,6 +152,7 @@ TEST(cpu_feed_forward, Contracts) {
   EXPECT_THROW(compute::gated_ffn(Xv, Wv, W2, Hv), compute::ValidationError);
   EXPECT_THROW(compute::gated_ffn(Xv, Wv, Wv, Hv), compute::ValidationError);
   EXPECT_THROW(compute::quantize_block(X, 64), compute::ValidationError);
+  EXPECT_THROW(compute::BlockScaled(4, 4, 0), compute::ValidationError);
 }
 
 int main(int argc, char** argv) { return mini_main(argc, argv); }

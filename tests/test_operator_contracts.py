@@ -144,6 +144,7 @@ def test_host_memory_is_refused(cb):
 def test_binding_checks_shapes_and_types(cb):
     import torch
     x, w, h = torch.zeros(4, 8).bfloat16(), torch.zeros(8, 6).bfloat16(), torch.zeros(4, 6).bfloat16()
+    q, c = torch.zeros(4, 16, dtype=torch.uint8), torch.zeros(4, 4)
     cases = [
         lambda: cb.gated_ffn(x, w, w, torch.zeros(4, 5).bfloat16(), stream=0),
         lambda: cb.gated_ffn(x, w, w.half(), h, stream=0),
@@ -157,6 +158,8 @@ def test_binding_checks_shapes_and_types(cb):
         lambda: cb.quantize_block(x, torch.zeros(4, 8, dtype=torch.uint8), torch.zeros(1, 1), stream=0),
         lambda: cb.quantize_block(x, torch.zeros(4, 8, dtype=torch.uint8), torch.zeros(4, 1), transpose=True, stream=0),
         lambda: cb.gemm_block_scaled(x, torch.zeros(4, 1), x, torch.zeros(1, 1), h, stream=0),
+        lambda: cb.gemm_block_scaled(q, torch.zeros(4, 1), q, torch.zeros(4, 1), c, bias=torch.zeros(3), stream=0),
+        lambda: cb.gemm_block_scaled(q, torch.zeros(4, 1), q, torch.zeros(4, 1), c, bias=torch.zeros(8)[::2], stream=0),
     ]
     for i, call in enumerate(cases):
         with pytest.raises(ValueError):
