@@ -60,6 +60,9 @@ struct BlockShape {
   static constexpr uint32_t kBStage = kBRows * kBlockK;
   static constexpr int kStages = 6;
   static constexpr int kBufs = 512 / BN;  // block accumulators in TMEM
+  // The epilogue follows a stage's barrier by its parity. The issuer runs at most
+  // kBufs k-blocks ahead of it, so the barrier may not come round sooner.
+  static_assert(kStages >= kBufs, "a stage's barrier would complete twice before the epilogue looks");
   // 256-column tiles are two MMAs of 128 columns with an accumulator each: half
   // h is 64 columns of each CTA's B rows, tile columns 64 h .. and 128 + 64 h ..
   // The two epilogue warps of an SM sub-partition take one half each, so they

@@ -160,6 +160,9 @@ struct SkinnyShape {
   static constexpr uint32_t kRing = kStages * (kWStage + kXStage);
   static constexpr int kSmem = static_cast<int>(kRing) + 1024 + 256;
   static_assert(NT * 128 * 4 <= kRing, "the partial sums reuse the ring");
+  // kBlock: the epilogue follows a stage's barrier by its parity. The issuer runs
+  // at most kBufs k-blocks ahead of it, so the barrier may not come round sooner.
+  static_assert(kStages >= kBufs, "a stage's barrier would complete twice before the epilogue looks");
   static_assert(2 * (kSmem + 1024) <= 228 * 1024, "two CTAs an SM");
 };
 
