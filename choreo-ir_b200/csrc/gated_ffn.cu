@@ -25,11 +25,6 @@ template <bool W_MN, typename OutT, bool GRAD>
 int dispatch_tile(const TcConfig& cfg, const CUtensorMap& ta, const TwoMaps& tb, const GateMaps& tc,
                   const GateParams& kp, int grid, cudaStream_t s) {
   using Epi = GateEpi<OutT, GRAD>;
-  if (cfg.wide) {
-    static std::atomic<uint64_t> done{0};
-    return launch_tiles(tc_gemm_pair_wide_kernel<kWideStages, GateLoader<W_MN, 128, true>, Epi>,
-                        tc_wide_smem_bytes<kWideStages>(), done, ta, tb, tc, kp, grid, s);
-  }
   if (cfg.pair) {
     constexpr int ST = pair_stages_for(256);
     static std::atomic<uint64_t> done{0};
@@ -97,10 +92,12 @@ int fill_tc_params(TcParams* kp, int64_t m, int64_t n, int64_t tiles_n, int64_t 
 
 TcConfig select_gate_config(int64_t m, int64_t n, int64_t k) {
   // A tile of BN accumulator columns covers BN/2 columns of H: the GEMM cost
-  // model for M x 2N x K, among the shapes the gate kernels are built for.
-  return plan_tiles(m, 2 * n, (k + kBK - 1) / kBK, 1, current_sm_count(), false, 2,
-                    kTileWide256 | kTilePair256 | kTileSingle128)
-      .cfg;
+  // model for M x 2N x K, among the shapes the gate kernels are built for. The
+  // 512 x 256 pair tile is not: its epilogue spilled registers, and it took 204 us
+  // against the 256 x 256 tile's 170 at 4096 x 4096 x 4096, 137 against 114 at
+  // 1024 x 4096 x 10240, and on a loop of 8192 x 4096 x 10240 under the power cap
+  // 1120 against 1095.
+  return plan_tiles(m, 2 * n, (k + kBK - 1) / kBK, 1, current_sm_count(), false, 2, kTilePair256 | kTileSingle128).cfg;
 }
 
 namespace {
@@ -148,7 +145,7 @@ int launch_gate_tiles(const GateProblem& p, cudaStream_t stream) {
   TwoMaps tb;
   GateMaps tc;
   std::memset(&tc, 0, sizeof(tc));
-  int rc = encode_matrix(&ta, p.bf16, p.x, p.m, p.k, p.ldx, 64, cfg.wide ? 256u : 128u);
+  int rc = encode_matrix(&ta, p.bf16, p.x, p.m, p.k, p.ldx, 64, 128);
   if (rc) return rc;
   const uint32_t half = cfg.pair ? 128u : 64u;  // rows of one weight in the tile
   for (int i = 0; i < 2; ++i) {
@@ -316,7 +313,7 @@ int choreo_gated_ffn_query(const choreo_ffn_desc* d, choreo_launch_config* out) 
                                             : std::min<int64_t>(out->tiles, sms));
   out->block_x = kTcThreads;
   out->smem_bytes = c.smem;
-  out->tmem_cols = c.wide ? 512 : 2 * c.bn;
+  out->tmem_cols = 2 * c.bn;
   return ok();
 }
 

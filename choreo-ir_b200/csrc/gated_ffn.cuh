@@ -124,18 +124,6 @@ struct GateLoader {
     load3<PAIR>(dst_a, ta, bar, kb * kBK, m0, 0, pol_a);
     issue_b(tb, n0, kb, dst_b, bar, pol_b);
   }
-  struct WideCursor {
-    int m0, n0;
-  };
-  __device__ __forceinline__ static WideCursor wide_cursor(const TcParams&, int, int m0, int n0) {
-    return WideCursor{m0, n0};
-  }
-  __device__ __forceinline__ static void issue_wide(const CUtensorMap* ta, const TwoMaps* tb, const TcParams&,
-                                                    WideCursor& c, int kb, uint32_t dst_a, uint32_t dst_b,
-                                                    uint32_t bar, uint64_t pol_a, uint64_t pol_b) {
-    load3<PAIR>(dst_a, ta, bar, kb * kBK, c.m0, 0, pol_a);
-    issue_b(tb, c.n0, kb, dst_b, bar, pol_b);
-  }
 };
 
 struct SelectParams : TcParams {

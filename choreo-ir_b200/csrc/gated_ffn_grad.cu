@@ -104,6 +104,12 @@ using namespace choreo_sm100;
 namespace {
 
 constexpr unsigned kSelectTiles = kTileWide256 | kTilePair256 | kTileSingle128;
+// The 256 x 256 pair tile runs these products as fast as the wide one where both
+// need the same number of rounds, so the cost model gives them nearly one rate
+// (wide256's is 1.21) and the rounds decide: dWg and dWu at 2049 x 2048 x 5632,
+// six rounds of half tiles wide and five in pairs, 93 and 86 us; dX at 4096 x
+// 2048 x 5632, two either way, 160 and 165.
+constexpr double kPairRate = 1.15;
 
 template <typename Kern>
 int launch_select(Kern kern, int smem, std::atomic<uint64_t>& attr_done, const TwoMaps& ta, const TwoMaps& tb,
@@ -223,8 +229,8 @@ GradPlan plan_grad(const choreo_ffn_grad_desc& d) {
   if (d.dx != nullptr) {
     const int64_t kb = 2 * ((d.n + kBK - 1) / kBK);
     const int sms = current_sm_count();
-    g.dx = plan_tiles(d.m, d.k, kb, 1, sms, true, 2, kSelectTiles);
-    g.dx_unsplit = g.dx.split > 1 ? plan_tiles(d.m, d.k, kb, 1, sms, false, 2, kSelectTiles).cfg : g.dx.cfg;
+    g.dx = plan_tiles(d.m, d.k, kb, 1, sms, true, 2, kSelectTiles, kPairRate);
+    g.dx_unsplit = g.dx.split > 1 ? plan_tiles(d.m, d.k, kb, 1, sms, false, 2, kSelectTiles, kPairRate).cfg : g.dx.cfg;
     if (g.dx.split > 1) {
       g.partials = g.bytes;
       g.bytes += round_up(g.dx.split * d.m * d.k * 4, 256);
@@ -276,7 +282,7 @@ int launch_dw(const choreo_ffn_grad_desc& d, int64_t n_pad, const void* dg, cons
   const int64_t rows = d.trans_w ? d.n : d.k, cols = d.trans_w ? d.k : d.n;
   const int64_t kb = (d.m + kBK - 1) / kBK;
   const TcConfig cfg =
-      plan_tiles(rows, cols, kb, 2, current_sm_count(), false, dtype_bytes(d.dtype_dw), kSelectTiles).cfg;
+      plan_tiles(rows, cols, kb, 2, current_sm_count(), false, dtype_bytes(d.dtype_dw), kSelectTiles, kPairRate).cfg;
   TwoMaps ta, tb, tc;
   int rc;
   for (int i = 0; i < 2; ++i) {

@@ -215,7 +215,7 @@ TcConfig make_config(bool pair, bool wide, int bn) {
 }  // namespace
 
 TilePlan plan_tiles(int64_t m, int64_t n, int64_t k_blocks, int64_t batch, int sm_count, bool allow_split,
-                    int out_bytes, unsigned tiles_built) {
+                    int out_bytes, unsigned tiles_built, double pair256_rate) {
   // Candidates: wide CTA pairs (512 x 256 tiles on 2 SMs), CTA pairs
   // (256 x BN) and single CTAs (128 x BN). A tile puts rows_per_sm x BN
   // outputs on each SM, `area` = rows_per_sm * BN / (128 * 256) slabs. One
@@ -237,7 +237,7 @@ TilePlan plan_tiles(int64_t m, int64_t n, int64_t k_blocks, int64_t batch, int s
   // bytes at about 5 TB/s plus a launch. The cheapest (tile, split) wins.
   struct Cand { const char* name; bool pair, wide; int bn; double eff, fixed, epi; };
   const Cand cands[6] = {{"wide256", true, true, 256, 1.21, 3.3, 4.1},
-                         {"pair256", true, false, 256, 1.01, 2.3, 4.4},
+                         {"pair256", true, false, 256, pair256_rate, 2.3, 4.4},
                          {"single256", false, false, 256, 0.89, 2.5, 2.2},
                          {"pair128", true, false, 128, 0.55, 1.3, 5.7},
                          {"single128", false, false, 128, 0.61, 1.4, 5.6},

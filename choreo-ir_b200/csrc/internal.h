@@ -118,7 +118,8 @@ inline int tile_rows_of(const TcConfig& c) { return c.wide ? 512 : (c.pair ? 256
 TcConfig select_tile_config(int64_t m, int64_t n, int64_t k_blocks, int64_t batch, int sm_count);
 // The tile shape and, with allow_split (batch 1), the number of K splits with
 // the lowest estimated time; out_bytes is the size of one output element.
-// tiles_built: which tile shapes the caller's kernel is built for (kTile* bits).
+// tiles_built: which tile shapes the caller's kernel is built for (kTile* bits);
+// pair256_rate: the pair256 tile's rate in the cost model's units.
 constexpr unsigned kTileWide256 = 1u << 0, kTilePair256 = 1u << 1, kTileSingle256 = 1u << 2, kTilePair128 = 1u << 3,
                    kTileSingle128 = 1u << 4, kTileSingle64 = 1u << 5, kAllTiles = (1u << 6) - 1;
 struct TilePlan {
@@ -127,7 +128,7 @@ struct TilePlan {
   double est_us = 0;
 };
 TilePlan plan_tiles(int64_t m, int64_t n, int64_t k_blocks, int64_t batch, int sm_count, bool allow_split,
-                    int out_bytes, unsigned tiles_built = kAllTiles);
+                    int out_bytes, unsigned tiles_built = kAllTiles, double pair256_rate = 1.01);
 
 // A GEMM with every operand already TMA-legal (16-byte aligned base, ld and
 // batch stride), in the orientation it is stored.
