@@ -16,10 +16,10 @@
 //                 (dWg and dWu: one launch, so one part-empty last wave).
 //
 // Bound by the tensor cores (and, on long calls, the 1 kW cap): 8192 x 4096 x
-// 10240 bf16 forward 1301k cycles, with G and U kept 1359k, the plain product
-// of the same size 1264k, the MMAs alone 1133k; dX 1230k, dWg with dWu 1247k.
-// The forward call takes 1.09-1.11 ms back to back, the backward pass with G
-// and U computed again 3.26-3.31 ms.
+// 10240 bf16 forward 1164k cycles, with G and U kept 1218k, the plain product
+// of the same size 1256k (1204k in the same tiles), the MMAs alone 1133k. The
+// forward call takes 1.08-1.10 ms back to back, the backward pass with G and U
+// computed again 3.21-3.27 ms.
 #pragma once
 #include "../../include/choreo_b200.h"
 #include "tc_kernel.cuh"
