@@ -5,7 +5,7 @@
 //   dG = dH * U * act'(G),  dU = dH * act(G)
 //   dX = dG Wg^T + dU Wu^T,  dWg = X^T dG,  dWu = X^T dU
 //
-// Three loaders feed the mainloops:
+// Two loaders feed the mainloops:
 //   GateLoader    B tile = the same BN/2 columns of Wg and of Wu, so a tile's
 //                 accumulator holds G in its first BN/2 columns and U in the
 //                 others and the product needs no second kernel and no memory
