@@ -214,6 +214,28 @@ def _stream_ptr(stream) -> int | None:
     return stream.cuda_stream
 
 
+def _workspace(need, workspace, device, stream):
+    """(tensor, bytes): the caller's workspace, or one of `need` bytes.
+
+    Memory allocated here comes from the call's own stream: torch's allocator
+    then orders it with that stream both ways. Memory of the current stream may
+    have been freed on the host while that stream's pending work still uses it,
+    and the call's stream does not wait for that work."""
+    if workspace is None:
+        if not need:
+            return None, 0
+        import torch
+        if stream is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        else:
+            if isinstance(stream, int):
+                # 0 and 1 are handles of the legacy default stream
+                stream = torch.cuda.ExternalStream(stream) if stream > 1 else torch.cuda.default_stream()
+            with torch.cuda.stream(stream):
+                workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    return workspace, workspace.numel() * workspace.element_size()
+
+
 def make_gemm_desc(a, b, c, *, m, n, k, trans_a=False, trans_b=False, lda=None, ldb=None, ldc=None,
                    alpha=1.0, beta=0.0, bias=None, relu=False, batch=1,
                    stride_a=0, stride_b=0, stride_c=0, dtype_ab=None, dtype_c=None, dtype_bias=None) -> GemmDesc:
@@ -267,14 +289,8 @@ def gemm(a, b, c, *, trans_a=False, trans_b=False, alpha=1.0, beta=0.0, bias=Non
     d = make_gemm_desc(a, b, c, m=m, n=n, k=k, trans_a=trans_a, trans_b=trans_b,
                        lda=a2.stride(0), ldb=b2.stride(0), ldc=c2.stride(0), alpha=alpha, beta=beta,
                        bias=bias, relu=relu, batch=batch, stride_a=sa, stride_b=sb, stride_c=sc)
-    ws_bytes = 0
-    if workspace is None:
-        need = gemm_query(d).workspace_bytes
-        if need:
-            import torch
-            workspace = torch.empty(need, dtype=torch.uint8, device=c.device)
-    if workspace is not None:
-        ws_bytes = workspace.numel() * workspace.element_size()
+    need = gemm_query(d).workspace_bytes if workspace is None else 0
+    workspace, ws_bytes = _workspace(need, workspace, c.device, stream)
     gemm_desc(d, workspace, ws_bytes, stream)
 
 
@@ -467,20 +483,6 @@ def _act_code(act):
     if act not in _ACTS:
         raise ValueError(f"unknown activation {act!r}: one of {', '.join(_ACTS)}")
     return _ACTS[act]
-
-
-def _workspace(need, workspace, device, stream):
-    """(tensor, bytes): the caller's workspace, or one of `need` bytes. Memory
-    allocated here belongs to torch's current stream: where the call runs on
-    another one, it is not handed out again before that one has passed the call."""
-    if workspace is None:
-        if not need:
-            return None, 0
-        import torch
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-        if stream is not None:
-            workspace.record_stream(torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream)
-    return workspace, workspace.numel() * workspace.element_size()
 
 
 def _pair_ld(a, b, rows, cols, names, like):
