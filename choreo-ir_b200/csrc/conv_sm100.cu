@@ -306,6 +306,7 @@ int launch_conv_tc(const choreo_conv_desc& d, cudaStream_t stream) {
     int rc = encode_tmap(&tc, cdt, 3, d.output, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
     kp.c_tma = 1;
+    kp.n_bulk = bulk_columns(d.k, ob);
   }
   kp.bias = d.bias;
   kp.dtype_bias = d.dtype_bias;

@@ -164,10 +164,9 @@ int encode_outputs(SelectParams* kp, TwoMaps* tc, int dtype_c, void* c0, void* c
   bool legal = (ld * eb) % 16 == 0 && (items == 1 || (stride * eb) % 16 == 0);
   for (void* c : {c0, c1})
     if (reinterpret_cast<uintptr_t>(c) & 15u) legal = false;
-  kp->c_vec_ok = legal ? 1 : 0;
-  // A bulk tensor store clips columns in whole 16 bytes: not where the rows end inside 16 bytes.
-  kp->c_tma = legal && (cols * eb) % 16 == 0 ? 1 : 0;
+  kp->c_vec_ok = kp->c_tma = legal ? 1 : 0;
   if (kp->c_tma == 0) return CHOREO_OK;
+  kp->n_bulk = bulk_columns(cols, eb);
   const CUtensorMapDataType dt = dtype_c == CHOREO_DTYPE_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                  : dtype_c == CHOREO_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                                 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;

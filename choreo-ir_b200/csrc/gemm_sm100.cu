@@ -352,12 +352,11 @@ int launch_gemm_tc(const TcProblem& p, const TcConfig& cfg, cudaStream_t stream)
   kp.relu = p.relu;
   // The kernels store C through a staging tile and bulk tensor stores when C
   // is TMA-addressable (16-byte aligned base, leading dimension and batch
-  // stride) and its rows end on a 16-byte boundary: a bulk tensor store clips
-  // columns in whole 16 bytes, so it would write past a row that ends inside.
+  // stride).
   CUtensorMap tc;
   std::memset(&tc, 0, sizeof(tc));
   kp.c_tma = 0;
-  if (kp.c_vec_ok && (p.n * cb) % 16 == 0) {
+  if (kp.c_vec_ok) {
     const uint64_t elem = static_cast<uint64_t>(cb);
     const uint64_t dims[3] = {static_cast<uint64_t>(p.n), static_cast<uint64_t>(p.m), static_cast<uint64_t>(items)};
     const uint64_t bstride = items > 1 ? static_cast<uint64_t>(p.stride_c) * elem
@@ -370,6 +369,7 @@ int launch_gemm_tc(const TcProblem& p, const TcConfig& cfg, cudaStream_t stream)
     int rc = encode_tmap(&tc, cdt, 3, p.c, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
     kp.c_tma = 1;
+    kp.n_bulk = bulk_columns(p.n, cb);
   }
   kp.status = status_word();
   kp.timeout_ns = wait_timeout_ns();

@@ -43,6 +43,13 @@ constexpr int stages_for(int bn) { return bn == 256 ? 4 : (bn == 128 ? 6 : 8); }
 constexpr int pair_stages_for(int bn) { return bn == 256 ? 6 : 8; }
 constexpr int kWideStages = 4;
 
+// Leading columns of an output that bulk tensor stores may write: all n, or,
+// where the rows end inside 16 bytes, the whole groups of 128 bytes (such a store
+// clips columns in whole 16 bytes and would write past the row).
+constexpr int32_t bulk_columns(int64_t n, int elem_bytes) {
+  return static_cast<int32_t>(n * elem_bytes % 16 == 0 ? n : n - n % (128 / elem_bytes));
+}
+
 // Everything the kernel needs besides the two tensor maps.
 struct TcParams {
   int32_t m, n;            // output rows / columns (per batch item)
@@ -59,6 +66,7 @@ struct TcParams {
   int64_t ldc, stride_c;   // elements
   int32_t c_vec_ok;        // 16-byte vector stores are legal for C
   int32_t c_tma;           // C is TMA-addressable: the epilogues store through staging tiles
+  int32_t n_bulk;          // with c_tma: columns stored in bulk (bulk_columns), the rest element by element
   float alpha, beta;
   const void* bias;
   int32_t dtype_bias;      // 8 f16, 9 f32, 11 bf16
@@ -262,6 +270,16 @@ __device__ __forceinline__ void stage_row_32(const float (&v)[32], uint32_t row_
   }
 }
 
+__device__ __forceinline__ uint16_t ld_shared_u16(uint32_t addr) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t ld_shared_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ float4 ld_shared_v4_f32(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
@@ -365,22 +383,49 @@ __device__ __forceinline__ void epilogue_chunk(const uint32_t (&r)[32], OutT* cr
     if (n_base + i < p.n) crow[n_base + i] = from_f32<OutT>(v[i]);
 }
 
+// The columns past n_bulk: the warp copies its staged rows (32 x 128 bytes,
+// 128-byte swizzle) element by element, neighbouring lanes in neighbouring columns.
+template <typename OutT>
+__device__ __forceinline__ void store_staged_tail(const TcParams& p, uint32_t stage_buf, int n_base, int row0, int b,
+                                                  int lane) {
+  __syncwarp();  // every lane has staged its row
+  OutT* dst = static_cast<OutT*>(p.c) + static_cast<int64_t>(b) * p.stride_c + static_cast<int64_t>(row0) * p.ldc +
+              n_base;
+  const int rows = min(32, p.m - row0), cols = p.n - n_base;
+#pragma unroll 1
+  for (int r = 0; r < rows; ++r, dst += p.ldc) {
+#pragma unroll 1
+    for (int c = lane; c < cols; c += 32) {
+      const uint32_t byte = static_cast<uint32_t>(c) * static_cast<uint32_t>(sizeof(OutT));
+      const uint32_t at = stage_buf + static_cast<uint32_t>(r) * 128u +
+                          ((((byte >> 4) ^ static_cast<uint32_t>(r & 7)) << 4) | (byte & 15u));
+      if constexpr (sizeof(OutT) == 2)
+        reinterpret_cast<uint16_t*>(dst)[c] = ld_shared_u16(at);
+      else
+        reinterpret_cast<uint32_t*>(dst)[c] = ld_shared_u32(at);
+    }
+  }
+  __syncwarp();  // the buffer may be staged again
+}
+
 // Epilogue of one warp: 32 accumulator rows (the TMEM lanes of the warp's
 // quarter) x kCols columns at TMEM address `taddr`, written to output rows
 // row0 .. row0 + 31 and columns n_first .. n_first + kCols of batch item b.
 // `release` hands the accumulator back to the MMA issuer, which waits for it
 // before the next tile's MMAs into the same columns, so the work before it is
 // on the MMA pipe's critical path.
-//  - 16-bit output through the TMA store without a beta * C term (the common
-//    case): every column is read from TMEM, scaled, biased (bias prefetched in
-//    `br`), clamped and packed to 16-bit pairs in registers, then the
-//    accumulator is released, and only then are the rows staged in the warp's
-//    4 KB buffer and sent as bulk tensor stores of 128-byte rows (clipped by
+//  - 16-bit output through the TMA store without a beta * C term and without
+//    columns past n_bulk (the common case): every column is read from TMEM,
+//    scaled, biased (bias prefetched in `br`), clamped and packed to 16-bit
+//    pairs in registers, then the accumulator is released, and only then are
+//    the rows staged in the warp's 4 KB buffer and sent as bulk tensor stores of 128-byte rows (clipped by
 //    the tensor map at the matrix edges).
 //  - otherwise columns are read in batches of 64 (two tcgen05.ld per wait),
 //    the accumulator is released once the last batch is in registers, and the
 //    arithmetic and stores follow batch by batch (staging + bulk tensor stores
-//    when C is TMA-addressable, else 16-byte vector stores).
+//    when C is TMA-addressable, element by element past n_bulk; else 16-byte
+//    vector stores). A tail in the first form kept its packed columns in
+//    registers longer and cost 16384 x 16384 x 128 four percent.
 template <int kCols, typename OutT, typename Release>
 __device__ __forceinline__ void epilogue_warp(uint32_t taddr, int n_first, int row0, int b, const TcParams& p,
                                               const CUtensorMap* tma_c, uint32_t stage_buf, int lane,
@@ -402,7 +447,7 @@ __device__ __forceinline__ void epilogue_warp(uint32_t taddr, int n_first, int r
   }
   const bool use_tma = kTmaOk && p.c_tma != 0;
   if constexpr (sizeof(OutT) == 2 && kTmaOk) {
-    if (use_tma && p.beta == 0.f) {
+    if (use_tma && p.beta == 0.f && min(n_first + kCols, p.n) <= p.n_bulk) {
       constexpr int kChunks = kCols / 32;
       const bool has_bias = p.bias != nullptr;
       if (has_bias) {
@@ -479,6 +524,10 @@ __device__ __forceinline__ void epilogue_warp(uint32_t taddr, int n_first, int r
             epilogue_values<OutT>(r[g * kCpg + c], v, crow, n_base + c * 32, p, row_ok, lane);
             stage_row_32<OutT>(v, stage_buf + static_cast<uint32_t>(lane) * 128u, lane,
                                c * (32 * static_cast<int>(sizeof(OutT)) / 16));
+          }
+          if (n_base >= p.n_bulk) {  // warp-uniform
+            store_staged_tail<OutT>(p, stage_buf, n_base, row0, b, lane);
+            break;
           }
           fence_proxy_async_smem();
           __syncwarp();
