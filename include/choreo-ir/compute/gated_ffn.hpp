@@ -145,7 +145,7 @@ Tensor<T> gated_ffn(const Tensor<T>& X, const Tensor<T>& Wg, const Tensor<T>& Wu
 template <typename T, typename TW = T>
 struct GatedFfnGrads {
   Tensor<T>* dX = nullptr;
-  Tensor<TW>* dWg = nullptr;   // laid out like the weights
+  Tensor<TW>* dWg = nullptr;   // laid out like the weights' storage: K x N, or N x K for transpose() views of it
   Tensor<TW>* dWu = nullptr;
   Tensor<T>* H = nullptr;
   const Tensor<T>* gate = nullptr;
@@ -153,12 +153,16 @@ struct GatedFfnGrads {
   bool accumulate = false;     // add to what dWg and dWu hold
 };
 
-/// Gradients of gated_ffn from dH (choreo_gated_ffn_backward). The weights
-/// are row-major K x N here.
-template <typename T, typename TW>
-void gated_ffn_backward(const Tensor<T>& dH, const Tensor<T>& X, const Tensor<T>& Wg, const Tensor<T>& Wu,
-                        const GatedFfnGrads<T, TW>& out, const GatedFfnConfig& cfg = GatedFfnConfig()) {
+/// Gradients of gated_ffn from dH (choreo_gated_ffn_backward). Operands as in
+/// gated_ffn: tensors or views, the weights row-major K x N or as transpose()
+/// views of N x K storage.
+template <typename T, typename TW, typename VD, typename VX, typename VG, typename VU>
+void gated_ffn_backward(const VD& dH, const VX& X, const VG& Wg, const VU& Wu, const GatedFfnGrads<T, TW>& out,
+                        const GatedFfnConfig& cfg = GatedFfnConfig()) {
   static_assert(std::is_same_v<T, float16_t> || std::is_same_v<T, bfloat16_t>, "gated_ffn needs f16 or bf16");
+  static_assert(std::is_same_v<T, detail::element_t<VD>> && std::is_same_v<T, detail::element_t<VX>> &&
+                    std::is_same_v<T, detail::element_t<VG>> && std::is_same_v<T, detail::element_t<VU>>,
+                "gated_ffn_backward: one element type");
   static_assert(std::is_same_v<TW, T> || std::is_same_v<TW, float>, "weight gradients: the weights' type or float");
   const char* what = "gated_ffn_backward";
   if (X.ndims() != 2) throw ValidationError("gated_ffn_backward: X must be 2-D");
@@ -166,13 +170,13 @@ void gated_ffn_backward(const Tensor<T>& dH, const Tensor<T>& X, const Tensor<T>
   d.m = X.shape()[0];
   d.k = X.shape()[1];
   const detail::FfnWeights w = detail::ffn_weights(Wg, Wu, d.k, what);
-  if (w.trans) throw ValidationError("gated_ffn_backward: the weights must be row-major");
   d.n = Wg.shape()[1];
   d.dtype = choreo_ir::detail::abi_dtype<T>();
   d.dtype_dw = choreo_ir::detail::abi_dtype<TW>();
   d.act = static_cast<int32_t>(cfg.activation);
   d.ldx = detail::row_major(X, d.m, d.k, what, "X");
   d.ldw = w.ld;
+  d.trans_w = w.trans ? 1 : 0;
   d.ld_dh = detail::row_major(dH, d.m, d.n, what, "dH");
   d.x = X.data();
   d.w_gate = Wg.data();
@@ -188,8 +192,9 @@ void gated_ffn_backward(const Tensor<T>& dH, const Tensor<T>& X, const Tensor<T>
   d.gate = optional(out.gate, d.m, d.n, "gate", &d.ld_gu);
   d.up = optional(out.up, d.m, d.n, "up", &d.ld_gu);
   d.dx = optional(out.dX, d.m, d.k, "dX", &d.ld_dx);
-  d.dw_gate = optional(out.dWg, d.k, d.n, "dWg", &d.ld_dw);
-  d.dw_up = optional(out.dWu, d.k, d.n, "dWu", &d.ld_dw);
+  const index_t w_rows = w.trans ? d.n : d.k, w_cols = w.trans ? d.k : d.n;
+  d.dw_gate = optional(out.dWg, w_rows, w_cols, "dWg", &d.ld_dw);
+  d.dw_up = optional(out.dWu, w_rows, w_cols, "dWu", &d.ld_dw);
   d.h = optional(out.H, d.m, d.n, "H", &d.ldh);
   d.accumulate_dw = out.accumulate ? 1 : 0;
   choreo_launch_config q;
