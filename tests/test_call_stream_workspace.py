@@ -153,3 +153,36 @@ def test_pending_work_on_freed_memory_is_left_alone(cb, cuda, op, raw):
         assert torch.equal(out, ref), i
         for dst in kept[i]:
             assert (dst == 17 + i).all(), i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["gemm", "gated_ffn", "gated_ffn_backward"])
+@pytest.mark.parametrize("raw", [False, True])
+def test_captured_on_a_joined_stream(cb, cuda, op, raw):
+    """A graph whose calls run on a second stream that joined the capture: the
+    workspaces are the graph's, and two graphs replayed in turn with new
+    allocations between them keep their results."""
+    import torch
+    run, shape = _problem(op)
+    ref = torch.empty(*shape, device="cuda", dtype=torch.bfloat16)
+    run(cb, ref, None)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    graphs = []
+    for _ in range(2):
+        out, graph = torch.zeros_like(ref), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            side.wait_stream(torch.cuda.current_stream())
+            for _ in range(2):
+                run(cb, out, side.cuda_stream if raw else side)
+            torch.cuda.current_stream().wait_stream(side)
+        graphs.append((graph, out))
+    for _ in range(3):
+        for graph, out in graphs:
+            out.zero_()
+            graph.replay()
+            torch.full((8 << 20,), 0x7F, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    cb.sync_status()
+    for _, out in graphs:
+        assert torch.equal(out, ref)
