@@ -225,7 +225,7 @@ def _workspace(need, workspace, device, stream):
         if not need:
             return None, 0
         import torch
-        if stream is None:
+        if stream is None or _stream_ptr(stream) == _stream_ptr(None):
             workspace = torch.empty(need, dtype=torch.uint8, device=device)
         else:
             if isinstance(stream, int):

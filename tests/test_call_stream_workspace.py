@@ -101,6 +101,12 @@ def test_workspace_without_a_stream_is_the_current_streams(cb, recorder, op):
     assert recorder.asked == ["current"] and recorder.ran == [0x77]
 
 
+@pytest.mark.parametrize("op", ["gemm", "gated_ffn", "gated_ffn_backward"])
+def test_workspace_of_the_current_stream_by_handle(cb, recorder, op):
+    calls(cb)[op](0x77)
+    assert recorder.asked == ["current"] and recorder.ran == [0x77]
+
+
 def _problem(op):
     """(run(cb, out, stream), out shape and type, workspace bytes) of a call that needs a workspace."""
     import torch
