@@ -93,10 +93,9 @@ int fill_tc_params(TcParams* kp, int64_t m, int64_t n, int64_t tiles_n, int64_t 
 TcConfig select_gate_config(int64_t m, int64_t n, int64_t k) {
   // A tile of BN accumulator columns covers BN/2 columns of H: the GEMM cost
   // model for M x 2N x K, among the shapes the gate kernels are built for. The
-  // 512 x 256 pair tile is not: its epilogue spilled registers, and it took 204 us
-  // against the 256 x 256 tile's 170 at 4096 x 4096 x 4096, 137 against 114 at
-  // 1024 x 4096 x 10240, and on a loop of 8192 x 4096 x 10240 under the power cap
-  // 1120 against 1095.
+  // 512 x 256 pair tile is not: it took 204 us against the 256 x 256 tile's 170 at
+  // 4096 x 4096 x 4096, 137 against 114 at 1024 x 4096 x 10240, and on a loop of
+  // 8192 x 4096 x 10240 under the power cap 1120 against 1095.
   return plan_tiles(m, 2 * n, (k + kBK - 1) / kBK, 1, current_sm_count(), false, 2, kTilePair256 | kTileSingle128).cfg;
 }
 

@@ -18,8 +18,8 @@
 // Bound by the tensor cores (and, on long calls, the 1 kW cap): 8192 x 4096 x
 // 10240 bf16 forward 1164k cycles, with G and U kept 1218k, the plain product
 // of the same size 1256k (1204k in the same tiles), the MMAs alone 1133k. The
-// forward call takes 1.08-1.10 ms back to back, the backward pass with G and U
-// computed again 3.21-3.27 ms.
+// forward call takes 1.06-1.10 ms back to back, the backward pass with G and U
+// computed again 3.16-3.27 ms.
 #pragma once
 #include "../../include/choreo_b200.h"
 #include "tc_kernel.cuh"
@@ -288,7 +288,11 @@ __device__ __forceinline__ void gate_pack(const uint32_t (&r)[kChunks][32], uint
 // Forward: h = act(G) * U from the fp32 accumulators, and G and U themselves
 // when they are kept. Backward (GRAD): dG and dU from G, U and dH, and h when
 // it is wanted again. A warp takes the same BN/4 columns of G and of U, read
-// from TMEM at once and handed back before the arithmetic.
+// from TMEM at once and handed back before the arithmetic. In the 256-column
+// tile these are 128 registers of a thread's 168 and the packed columns 32 more:
+// the forward form spills 244 bytes a thread (432 read back), GRAD, which takes
+// 32 columns at a time, 12 (16). What that costs is not measured; with it the
+// large product takes 1.03 of its MMAs' cycles.
 template <typename OutT, bool GRAD>
 struct GateEpi {
   using MapC = GateMaps;

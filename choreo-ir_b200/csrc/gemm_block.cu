@@ -12,8 +12,9 @@
 // k-block takes 512 cycles of MMAs and 729 in all (1334 with a scale per column,
 // which doubles the arithmetic: a product of the two scales and the sum for
 // every element), and on long calls by the 1 kW cap: 8192^3 with bf16 output
-// 539 us = 2.04 PFLOP/s, 4096^3 80 us, the f32 weight gradient 4096 x 10240 x
-// 8192 with both scales per row 570 us.
+// 536-546 us = 2.0 PFLOP/s, 4096^3 80 us, the f32 weight gradient 4096 x 8192 x
+// 10240 with both scales per row 566-586 us. That form spills 46 bytes a thread
+// (108 read back); the one with a scale per 128 rows does not.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

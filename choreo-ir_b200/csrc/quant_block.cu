@@ -5,9 +5,12 @@
 //   scale = a / 448,  q = e4m3(x * (448 / a)),  each step rounded to fp32
 //
 // Memory-bound: 2 or 4 bytes read and 1 written per element. 8192 x 10240 bf16
-// in rows 46 us = 0.84 of the copy bandwidth, transposed 48 us with either block;
-// f32 transposed 65 us (128 x 128) and 68 us (1 x 128) = 0.98 and 0.94; 8191 x
-// 4100 f32 in 128 x 128 blocks, transposed, 31.5 us = 0.81.
+// in rows 44-46 us = 0.84-0.88 of the copy bandwidth, in 128 x 128 blocks as they
+// lie 48 us = 0.79, transposed 47 us with either block; f32 in rows 71 us, in
+// 128 x 128 blocks 77 us, transposed 64 us (128 x 128) and 67 us (1 x 128) = 1.0
+// and 0.96; 8191 x 4100 f32 in 128 x 128 blocks, transposed, 30.6 us = 0.84.
+// Rows of X that are not 16-byte aligned are read element by element: 8192 x 10240
+// bf16 160 us in 128 x 128 blocks and 205 in 1 x 128, 8191 x 4100 f32 71 and 90.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

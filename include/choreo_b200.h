@@ -160,7 +160,9 @@ int choreo_sync_status(void* stream);
  * (compute/compute.hpp:32-44), which its dispatcher ignores. */
 typedef struct choreo_tuning {
   char tile[16];            /* "" = cost model; else force "wide256", "pair256", "pair128",
-                               "single256", "single128" or "single64" (GEMM and conv) */
+                               "single256", "single128" or "single64" (GEMM and conv; the gated
+                               product and its backward pass follow a shape that they are
+                               built for and take pair256 for another) */
   int32_t split_k;          /* 0 = cost model; n >= 1 = only plans with exactly n K ranges
                                (where K divides into them; else the unsplit plan) */
   int32_t group_m;          /* 0 = rasterise tiles in groups of 4096 rows of A;
@@ -184,7 +186,9 @@ int choreo_tuning_set(const choreo_tuning* t);
 int choreo_tuning_get(choreo_tuning* out);
 
 /* Measurement hook: while `probe` is set (non-NULL) on this host thread,
- * every tensor-core GEMM and conv launched from the thread adds, from its
+ * every tensor-core GEMM and conv (and every tile kernel of the gated and the
+ * block-scaled products, not their kernels for up to 128 rows) launched from the
+ * thread adds, from its
  * first CTA, the SM clock cycles (%clock64) and the global-timer nanoseconds
  * (%globaltimer) between that CTA's start and its end to probe[0] and
  * probe[1], and 1 to probe[2]: probe[0] / probe[1] is the effective SM clock
@@ -404,7 +408,9 @@ int choreo_quantize_block(const choreo_quant_desc* d, void* stream);
  * D is `addend` (M x N of C's type, ld_addend >= N), or C itself when it is
  * NULL; it is read only when beta != 0. bias and relu as in choreo_gemm_desc.
  * Each block's product is summed by the tensor cores and added to an fp32 sum
- * of all blocks. C is f16, bf16 or f32 and must not overlap the inputs. */
+ * of all blocks, times scale_a(i, t) * scale_b(j, t), which is rounded to fp32
+ * first: where that product is infinite so is the sum (or NaN, if the block's is
+ * 0). C is f16, bf16 or f32 and must not overlap the inputs. */
 typedef struct choreo_gemm_block_desc {
   int64_t m, n, k;
   const void* a;
